@@ -61,7 +61,10 @@ def _headers_mtime() -> float:
     return m
 
 
-COMMON_FLAGS = ["-O3", "-fPIC", "-std=c++20", f"--offload-arch={ARCH}", "-Wno-unused-result"]
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc -O3 forms them from ordinary float code, and some of
+# their forms have returned wrong results on this hardware now and then.  The host pass does not know the feature and says so.
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+COMMON_FLAGS = ["-O3", "-fPIC", "-std=c++20", f"--offload-arch={ARCH}", "-Wno-unused-result", *NO_PACKED_FP32]
 
 
 def _compile(src: str, verbose: bool, build_dir: str = BUILD, extra: tuple = ()) -> str:

@@ -2231,7 +2231,9 @@ constexpr bool persistent_kernel();
 template <int L, int E, typename OutT, int ACT>
 static void launch_pp_act(const GemmArgs& a0, hipStream_t s) {
   const int nb0 = (a0.M / BT_M) * (a0.N / PP_BN) * a0.ksplit;
-  if constexpr (persistent_kernel<L, E, OutT, ACT>()) {
+  // the persistent TN store into fp32 does not fit the register budget without packed fp32 math (256 B of scratch)
+  constexpr bool spills = L == L_TN && E == EPI_STORE && std::is_same<OutT, float>::value;
+  if constexpr (persistent_kernel<L, E, OutT, ACT>() && !spills) {
     GemmArgs a = a0;
     const int nb = grid_pp(a, nb0, a0.K / BT_K / a0.ksplit);
     if (a.tpb > 1) {
