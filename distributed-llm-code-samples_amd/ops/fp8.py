@@ -1,0 +1,307 @@
+"""Block-scaled 8-bit floating point: quantiser, read-back, matrix product and the linear layer on them.
+
+The reference trains in fp32 only (``linear_fwd`` / ``t_linear_bkwd``, train_ffns.py:41-45); this is the same three
+products with 8-bit operands, which the gfx950 matrix cores run at twice the bf16 rate.
+
+Format (``BlockFP8``): 8-bit codes (OCP e4m3 or e5m2) with one power-of-two scale per row and 128 consecutive k -- or per
+128x128 tile, the same byte repeated on the tile's rows.  For a block with largest finite magnitude ``amax``
+
+    e = the smallest integer >= -127 with amax <= FMAX * 2^e        (FMAX: e4m3 448, e5m2 57344)
+    code = x * 2^-e rounded to nearest even,   stands for code * 2^e,   scale byte = e + 127
+
+The division is exact, so every value is rounded once (by at most half a step: 2^-4 relative for normal e4m3 codes, 2^-3
+for e5m2) and nothing finite saturates.  Non-finite elements do not enter ``amax``: NaN stays NaN, +-inf stays inf in e5m2
+and becomes NaN in e4m3 (which has no infinity), and the rest of their block keeps its values.
+
+GPU tensors run ``csrc/fp8.hip``; CPU tensors run the torch forms below (tests, oracle).
+"""
+from __future__ import annotations
+
+import contextlib
+from typing import NamedTuple
+
+import torch
+
+from .. import _native
+from .activations import act_code, act_fwd, act_grad
+from .gemm import EPIS
+
+BLOCK = 128
+FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
+_CODES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+_TOP = {torch.float8_e4m3fn: 8, torch.float8_e5m2: 15}   # FMAX = 1.75 * 2^top
+
+
+class BlockFP8(NamedTuple):
+    """An 8-bit operand of logical shape ``[rows, k]``: ``data`` [rows, k rounded up to 128] (zeros behind ``k``) in a torch
+    float8 type, ``scale`` uint8 [k blocks, rows] (exponent bytes, biased by 127)."""
+    data: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    @property
+    def rows(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def device(self) -> torch.device:
+        return self.data.device
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _fmt(fmt: str) -> torch.dtype:
+    if fmt not in FORMATS:
+        raise ValueError(f"unknown 8-bit format {fmt!r}; choose from {sorted(FORMATS)}")
+    return FORMATS[fmt]
+
+
+def _on(device: torch.device):
+    """Launches go to the tensors' device, whichever device is current."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def fp8_empty(rows: int, k: int, fmt: str = "e4m3", device=None) -> BlockFP8:
+    """Storage for a ``[rows, k]`` operand (uninitialised), for the quantisers' ``out``."""
+    return BlockFP8(torch.empty((rows, _blocks(k) * BLOCK), dtype=_fmt(fmt), device=device),
+                    torch.empty((_blocks(k), rows), dtype=torch.uint8, device=device), k)
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Row stride of a row-major view (torch leaves the stride of a single row arbitrary)."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check(q: BlockFP8, name: str) -> None:
+    if q.data.dim() != 2 or q.data.dtype not in _CODES:
+        raise TypeError(f"{name}: data must be a 2-D float8 tensor (e4m3fn or e5m2), got {q.data.dtype} {tuple(q.data.shape)}")
+    if q.k < 0 or q.data.shape[1] != _blocks(q.k) * BLOCK:
+        raise ValueError(f"{name}: data of k = {q.k} has {_blocks(q.k) * BLOCK} columns, got {q.data.shape[1]}")
+    if q.scale.dtype != torch.uint8 or tuple(q.scale.shape) != (_blocks(q.k), q.data.shape[0]):
+        raise ValueError(f"{name}: scale must be uint8 {(_blocks(q.k), q.data.shape[0])}, got {q.scale.dtype} "
+                         f"{tuple(q.scale.shape)}")
+    if q.scale.device != q.data.device:
+        raise ValueError(f"{name}: data on {q.data.device}, scale on {q.scale.device}")
+    if q.data.numel() and (q.data.stride(1) != 1 or (q.scale.stride(1) != 1 and q.scale.shape[1] > 1)):
+        raise ValueError(f"{name}: data and scale must be contiguous along their last dimension")
+    if q.data.device.type == "cuda" and q.data.numel() and (q.data.data_ptr() % 16 or _ld(q.data) % 16):
+        raise ValueError(f"{name}: data rows must start at multiples of 16 bytes")
+
+
+def _pow2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32, exactly, for integer -127 <= e <= 127."""
+    normal = ((e + 127) << 23).to(torch.int32).view(torch.float32)
+    return torch.where(e == -127, torch.full_like(normal, 2.0 ** -127), normal)
+
+
+def _quantize_torch(x: torch.Tensor, dt: torch.dtype, tile: bool, out: BlockFP8) -> None:
+    R, K = x.shape
+    kb, rb = _blocks(K), _blocks(R)
+    p = torch.zeros((rb * BLOCK if tile else R, kb * BLOCK), dtype=torch.float32, device=x.device)
+    p[:R, :K] = x
+    v = p.view(rb, BLOCK, kb, BLOCK) if tile else p.view(R, 1, kb, BLOCK)
+    amax = torch.where(torch.isfinite(v), v.abs(), torch.zeros_like(v)).amax(dim=(1, 3), keepdim=True)
+    bits = amax.contiguous().view(torch.int32)
+    e = (((bits + 0x1FFFFF) >> 23) - _TOP[dt]).clamp(min=0) - 127
+    q = v * _pow2(-e)
+    if dt == torch.float8_e4m3fn:
+        q = torch.where(torch.isinf(q), torch.full_like(q, float("nan")), q)
+    out.data.copy_(q.reshape(p.shape)[:R].to(dt))
+    out.scale.copy_((e + 127).to(torch.uint8).expand(v.shape[0], v.shape[1], kb, 1).reshape(-1, kb)[:R].t())
+
+
+def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bool) -> None:
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
+    R, C = x.shape
+    for o, rows, k, name in ((q, R, C, "out"), (qt, C, R, "out_t")):
+        if o is None:
+            continue
+        _check(o, name)
+        if o.rows != rows or o.k != k or o.device != x.device:
+            raise ValueError(f"{name} must hold {(rows, k)} on {x.device}, got {(o.rows, o.k)} on {o.device}")
+    if R == 0 or C == 0:
+        return
+    if x.device.type != "cuda":
+        if q is not None:
+            _quantize_torch(x, q.data.dtype, tile, q)
+        if qt is not None:
+            _quantize_torch(x.t(), qt.data.dtype, tile, qt)
+        return
+    if x.stride(1) != 1 and C > 1:
+        x = x.contiguous()
+    null = (None, 0, None, 0)
+    arg = lambda o: null if o is None else (o.data.data_ptr(), _ld(o.data), o.scale.data_ptr(),  # noqa: E731
+                                            _ld(o.scale))
+    code = lambda o: 0 if o is None else _CODES[o.data.dtype]  # noqa: E731
+    with _on(x.device):
+        rc = _native.lib().dllm_fp8_quantize(x.data_ptr(), _native.dtype_code(x.dtype), x.stride(0), R, C, *arg(q), *arg(qt),
+                                             code(q), code(qt), int(tile), _native.stream_ptr(x.device))
+    _native.check(rc, f"dllm_fp8_quantize({R}x{C})")
+
+
+def quantize_fp8(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
+    """The 8-bit form of ``x`` [R, K] (bf16 / fp32), scaled per row and 128 columns (``tile``: per 128x128 tile)."""
+    if out is None:
+        out = fp8_empty(*_shape2(x), fmt, x.device)
+    _quantize(x, out, None, tile)
+    return out
+
+
+def quantize_fp8_t(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
+    """The 8-bit form of ``xᵀ`` [K, R], scaled per column of ``x`` and 128 rows (``tile``: per 128x128 tile)."""
+    if out is None:
+        out = fp8_empty(*reversed(_shape2(x)), fmt, x.device)
+    _quantize(x, None, out, tile)
+    return out
+
+
+def quantize_fp8_both(x: torch.Tensor, fmt: str = "e4m3", fmt_t: str = "e4m3", *, tile: bool = False,
+                      out: BlockFP8 | None = None, out_t: BlockFP8 | None = None) -> tuple[BlockFP8, BlockFP8]:
+    """``(quantize_fp8(x, fmt), quantize_fp8_t(x, fmt_t))`` from one read of ``x``: a forward (or input-gradient) operand
+    and the weight-gradient operand of the same tensor."""
+    R, C = _shape2(x)
+    out = fp8_empty(R, C, fmt, x.device) if out is None else out
+    out_t = fp8_empty(C, R, fmt_t, x.device) if out_t is None else out_t
+    _quantize(x, out, out_t, tile)
+    return out, out_t
+
+
+def _shape2(x: torch.Tensor) -> tuple[int, int]:
+    if x.dim() != 2:
+        raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
+    return x.shape[0], x.shape[1]
+
+
+def dequantize_fp8(q: BlockFP8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values ``[rows, k]`` that ``q`` stands for, in bf16 or fp32: exact but where the type ends (a code that rounded up
+    to 2^128 reads as inf; values among the type's subnormals are rounded)."""
+    _check(q, "q")
+    if out is None:
+        out = torch.empty((q.rows, q.k), dtype=dtype, device=q.device)
+    if tuple(out.shape) != (q.rows, q.k) or out.device != q.device or out.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"out must be bf16 or fp32 {(q.rows, q.k)} on {q.device}")
+    if q.rows == 0 or q.k == 0:
+        return out
+    if q.device.type != "cuda":
+        kb = _blocks(q.k)
+        e = q.scale.t().to(torch.int32) - 127
+        s = torch.where(e == 128, torch.full_like(e, 0), e)
+        v = q.data.float().view(q.rows, kb, BLOCK) * _pow2(s).unsqueeze(2)
+        v = torch.where((e == 128).unsqueeze(2), torch.full_like(v, float("nan")), v)
+        out.copy_(v.reshape(q.rows, -1)[:, :q.k])
+        return out
+    if out.stride(1) != 1 and q.k > 1:
+        raise ValueError("out must be row-major")
+    with _on(q.device):
+        rc = _native.lib().dllm_fp8_dequantize(q.data.data_ptr(), _ld(q.data), q.scale.data_ptr(), _ld(q.scale),
+                                               _CODES[q.data.dtype], out.data_ptr(), _native.dtype_code(out.dtype),
+                                               _ld(out), q.rows, q.k, _native.stream_ptr(q.device))
+    _native.check(rc, f"dllm_fp8_dequantize({q.rows}x{q.k})")
+    return out
+
+
+def _check_rows(t: torch.Tensor, name: str, shape: tuple, device) -> None:
+    if t.dim() != 2 or tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{name} must be {shape} on {device}, got {tuple(t.shape)} on {t.device}")
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name} must be a row-major view without overlapping rows, got strides {t.stride()}")
+
+
+def gemm_fp8(a: BlockFP8, b: BlockFP8, out: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16,
+             alpha: float = 1.0, beta: float = 0.0, epi: str = "store", act: str = "none",
+             aux: torch.Tensor | None = None, aux_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``C[M, N] = A[M, K] · B[N, K]ᵀ`` of two 8-bit operands (either format on either side), fp32 accumulation, bf16 or
+    fp32 ``out`` (any row stride).  Epilogues as in ``gemm``: ``"store"`` (``alpha·acc + beta·C``), ``"act"``
+    (``C = act(acc)``, ``aux_out = acc``) and ``"dact"`` (``C = acc · act'(aux)``)."""
+    _check(a, "a")
+    _check(b, "b")
+    if a.k != b.k:
+        raise ValueError(f"gemm_fp8: inner dims differ ({a.k} vs {b.k})")
+    if a.device != b.device:
+        raise ValueError(f"gemm_fp8: operands on {a.device} and {b.device}")
+    if epi not in ("store", "act", "dact"):
+        raise ValueError(f"gemm_fp8: unknown epilogue {epi!r}; choose from store, act, dact")
+    code = act_code(act)
+    if epi != "store" and act == "none":
+        raise ValueError(f"gemm_fp8: epilogue {epi} needs an activation")
+    if epi != "store" and (alpha != 1.0 or beta != 0.0):
+        raise ValueError(f"gemm_fp8: epilogue {epi} takes no alpha / beta")
+    M, N = a.rows, b.rows
+    if out is None:
+        if beta != 0.0:
+            raise ValueError("gemm_fp8: beta needs out")
+        out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    if out.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"gemm_fp8: out must be bf16 or fp32, got {out.dtype}")
+    _check_rows(out, "out", (M, N), a.device)
+    if epi == "dact" and aux is None:
+        raise ValueError("gemm_fp8: epilogue dact needs aux (pre-activation)")
+    if (aux is not None) != (epi == "dact") or (aux_out is not None and epi != "act"):
+        raise ValueError("gemm_fp8: aux belongs to epilogue dact, aux_out to act")
+    side = aux if aux is not None else aux_out
+    if side is not None:
+        _check_rows(side, "aux" if aux is not None else "aux_out", (M, N), a.device)
+        if side.dtype != out.dtype:
+            raise TypeError("gemm_fp8: aux / aux_out must have the output dtype")
+    if M == 0 or N == 0:
+        return out
+    if a.device.type != "cuda":
+        acc = dequantize_fp8(a) @ dequantize_fp8(b).t()
+        if epi == "store":
+            out.copy_(alpha * acc + beta * out.float() if beta != 0.0 else alpha * acc)
+        elif epi == "act":
+            if aux_out is not None:
+                aux_out.copy_(acc)
+            out.copy_(act_fwd(act, acc))
+        else:
+            out.copy_(acc * act_grad(act, aux.float()))
+        return out
+    with _on(a.device):
+        rc = _native.lib().dllm_fp8_gemm(
+            a.data.data_ptr(), _ld(a.data), a.scale.data_ptr(), _ld(a.scale), _CODES[a.data.dtype],
+            b.data.data_ptr(), _ld(b.data), b.scale.data_ptr(), _ld(b.scale), _CODES[b.data.dtype],
+            out.data_ptr(), _ld(out), _native.dtype_code(out.dtype), aux.data_ptr() if aux is not None else None,
+            aux_out.data_ptr() if aux_out is not None else None, _ld(side) if side is not None else 0, M, N, _blocks(a.k),
+            float(alpha), float(beta), EPIS[epi], code, _native.stream_ptr(a.device))
+    _native.check(rc, f"dllm_fp8_gemm({epi},M={M},N={N},K={a.k})")
+    return out
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# the linear layer on 8-bit operands
+# ----------------------------------------------------------------------------------------------------------------
+class LinearFP8(NamedTuple):
+    """What ``linear_fp8`` keeps for its backward: xᵀ (weight gradient) and wᵀ (input gradient) in 8 bits."""
+    x_t: BlockFP8
+    w_t: BlockFP8
+
+
+def linear_fp8(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, LinearFP8]:
+    """``y = x·wᵀ`` (``linear_fwd`` train_ffns.py:41-42) with x [T, D] quantised per row and 128 columns and w [F, D] per
+    128x128 tile, both e4m3.  Returns ``(y, saved)``; ``saved`` goes to ``linear_fp8_bwd``."""
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"linear_fp8: x [T, D] and w [F, D], got {tuple(x.shape)} and {tuple(w.shape)}")
+    xq, xt = quantize_fp8_both(x)
+    wq, wt = quantize_fp8_both(w, tile=True)
+    return gemm_fp8(xq, wq, out, out_dtype=out_dtype), LinearFP8(xt, wt)
+
+
+def linear_fp8_bwd(dy: torch.Tensor, saved: LinearFP8, dw: torch.Tensor | None = None, *, beta: float = 0.0,
+                   dx: torch.Tensor | None = None, need_dx: bool = True) -> tuple[torch.Tensor | None, torch.Tensor]:
+    """``(dx, dw) = (dy·w, dyᵀ·x)`` (``t_linear_bkwd`` train_ffns.py:44-45) with dy [T, F] quantised to e5m2 (gradients
+    need range more than digits): per row for dx, per column for dw.  ``dx`` has dy's type, ``dw`` is fp32 unless given;
+    ``beta`` accumulates into ``dw``."""
+    if dy.dim() != 2 or dy.shape != (saved.x_t.k, saved.w_t.k):
+        raise ValueError(f"linear_fp8_bwd: dy must be {(saved.x_t.k, saved.w_t.k)}, got {tuple(dy.shape)}")
+    if need_dx:
+        dq, dt = quantize_fp8_both(dy, "e5m2", "e5m2")
+        dx = gemm_fp8(dq, saved.w_t, dx, out_dtype=dy.dtype)
+    else:
+        dx, dt = None, quantize_fp8_t(dy, "e5m2")
+    return dx, gemm_fp8(dt, saved.x_t, dw, out_dtype=torch.float32, beta=beta)
