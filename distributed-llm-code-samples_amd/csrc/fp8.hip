@@ -2,6 +2,7 @@
 #include <type_traits>
 
 #include "fp8.h"
+#include "nt8.h"
 
 namespace dllm {
 
@@ -379,11 +380,201 @@ __global__ __launch_bounds__(256, 2) void fp8_gemm_128(Fp8GemmArgs p) {
       f8_epi4<EPI, OutT>(p, m0 + wr * 64 + i * 16 + i15, n0 + wc * 64 + k * 16 + 4 * g, acc[i][k]);
 }
 
+// ----------------------------------------------------------------------------------------------
+// 256x256 tiles on the 8-phase loop (nt8.h), one matrix instruction per 16x16 fragment pair and K step.
+//
+// Scales: a lane's four A rows of a half are consecutive rows of C (nt8.h), so one 32-bit word of the K step's scale row
+// holds them, and 16 bits its two B rows; the matrix instruction picks the byte (op_sel), so scaling costs two 4-byte and
+// two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more: the last step again, with scale
+// bytes 0 on both sides, 2^-254 of it, which leaves every fp32 sum as it is.
+// ----------------------------------------------------------------------------------------------
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+
+template <int FA, int FB>
+struct F8Trait {
+  const uint8_t *sa, *sb;      // scale bytes of K step 0
+  long ldsa, ldsb;
+  int nk, nk2;
+  uint32_t oa[2], ob[2];       // the lane's scale bytes in a scale row, per half
+  uint32_t sh;                 // right shifts of the four words, 8 bits each: words that would pass the row's end start
+                               // earlier (rows that far are never stored)
+  int keep;                    // 0 if the current pair's second step is the one behind the last
+  int wa[2][2], wb[2][2];      // [K step parity][half]; as loaded until the step's first phase shifts them
+
+  __device__ __forceinline__ void begin(const Fp8GemmArgs& p, int m0, int n0, int wid, int lane) {
+    sa = p.SA; sb = p.SB; ldsa = p.ldsa; ldsb = p.ldsb;
+    nk = p.nk; nk2 = (p.nk + 1) >> 1;
+    sh = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int ra = m0 + 128 * h + (wid >> 2) * 64 + 4 * (lane & 15), rb = n0 + 128 * h + (wid & 3) * 32 + 2 * (lane & 15);
+      oa[h] = (uint32_t)min(ra, p.M - 4);
+      ob[h] = (uint32_t)min(rb, p.N - 2);
+      sh |= (uint32_t)min(8 * (ra - (int)oa[h]), 24) << (8 * h) | (uint32_t)min(8 * (rb - (int)ob[h]), 8) << (16 + 8 * h);
+    }
+    fetch<0>(0);
+    fetch<1>(1);
+  }
+  __device__ __forceinline__ int step(int pair) const { return 2 * pair + 1 < nk ? 128 : 0; }
+  __device__ __forceinline__ int advance(const char*& an, const char*& bn, int it) {
+    keep = 2 * it + 1 < nk ? -1 : 0;
+    if (it + 1 < nk2) {
+      an += 256;
+      bn += 256;
+      return step(it + 1);
+    }
+    return step(it);
+  }
+  template <int ODD>
+  __device__ __forceinline__ void fetch(int kt) {
+    const int k = min(kt, nk - 1);
+    const uint8_t *a = sa + (long)k * ldsa, *b = sb + (long)k * ldsb;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      wa[ODD][h] = (int)*(const u32_any*)(a + oa[h]);
+      wb[ODD][h] = (int)*(const u16_any*)(b + ob[h]);
+    }
+  }
+  template <class ODD> __device__ __forceinline__ void load(ODD, int it) { fetch<ODD::value>(2 * it + 2 + ODD::value); }
+
+  template <int MT, int NT>
+  static __device__ __forceinline__ void one(f32x4_t& c, const N8Frag& fa, const N8Frag& fb, int a, int b) {
+    const i32x8_t x = __builtin_shufflevector(fa.lo, fa.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    const i32x8_t y = __builtin_shufflevector(fb.lo, fb.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x, c, FB, FA, NT, b, MT, a);
+  }
+  template <int QM, int QN, int ODD>
+  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], const N8Frag (&fa)[4], const N8Frag (&fb)[2]) {
+    if constexpr (QM == 0 && QN == 0) {   // the step's first phase
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        wa[ODD][h] = (int)((uint32_t)wa[ODD][h] >> (sh >> (8 * h) & 31));
+        wb[ODD][h] = (int)((uint32_t)wb[ODD][h] >> (sh >> (16 + 8 * h) & 31));
+        if constexpr (ODD) { wa[ODD][h] &= keep; wb[ODD][h] &= keep; }
+      }
+    }
+    const int a = wa[ODD][QM], b = wb[ODD][QN];
+    one<0, 0>(c[0][0], fa[0], fb[0], a, b); one<0, 1>(c[0][1], fa[0], fb[1], a, b);
+    one<1, 0>(c[1][0], fa[1], fb[0], a, b); one<1, 1>(c[1][1], fa[1], fb[1], a, b);
+    one<2, 0>(c[2][0], fa[2], fb[0], a, b); one<2, 1>(c[2][1], fa[2], fb[1], a, b);
+    one<3, 0>(c[3][0], fa[3], fb[0], a, b); one<3, 1>(c[3][1], fa[3], fb[1], a, b);
+  }
+};
+
+// 8 columns n .. n + 7 of row m; `fast`: the tile is inside C and rows are 16-byte aligned
+template <int EPI, typename OutT>
+__device__ __forceinline__ void f8_epi8(const Fp8GemmArgs& p, bool fast, int m, int n, const float (&v)[8]) {
+  if (!fast) {
+    f8_epi4<EPI, OutT>(p, m, n, f32x4_t{v[0], v[1], v[2], v[3]});
+    f8_epi4<EPI, OutT>(p, m, n + 4, f32x4_t{v[4], v[5], v[6], v[7]});
+    return;
+  }
+  auto load = [](const void* base, long i, float (&x)[8]) {
+    if constexpr (sizeof(OutT) == 2) {
+      const uint4 u = *(const uint4*)((const uint16_t*)base + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[2 * k] = __uint_as_float(w[k] << 16);
+        x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+      }
+    } else {
+      const f32x4_t a = *(const f32x4_t*)((const float*)base + i), b = *(const f32x4_t*)((const float*)base + i + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { x[k] = a[k]; x[4 + k] = b[k]; }
+    }
+  };
+  auto store = [](void* base, long i, const float (&x)[8]) {
+    if constexpr (sizeof(OutT) == 2) {
+      uint4 u;
+      u.x = f2bf(x[0]) | ((uint32_t)f2bf(x[1]) << 16); u.y = f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16);
+      u.z = f2bf(x[4]) | ((uint32_t)f2bf(x[5]) << 16); u.w = f2bf(x[6]) | ((uint32_t)f2bf(x[7]) << 16);
+      *(uint4*)((uint16_t*)base + i) = u;
+    } else {
+      *(f32x4_t*)((float*)base + i) = f32x4_t{x[0], x[1], x[2], x[3]};
+      *(f32x4_t*)((float*)base + i + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
+    }
+  };
+  const long i = (long)m * p.ldc + n, ia = (long)m * p.ldaux + n;
+  float o[8];
+  if constexpr (EPI == EPI_STORE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = v[e] * p.alpha;
+    if (p.beta != 0.f) {
+      float c[8];
+      load(p.C, i, c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += p.beta * c[e];
+    }
+  } else if constexpr (EPI == EPI_ACT) {
+    if (p.aux_out) store(p.aux_out, ia, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = act_fwd(p.act, v[e]);
+  } else {
+    float h[8];
+    load(p.aux, ia, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = v[e] * act_grad(p.act, h[e]);
+  }
+  store(p.C, i, o);
+}
+
+template <int EPI, typename OutT, int FA, int FB>
+__global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[N8_LDS];
+  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int tiles_m = (p.M + 255) >> 8, tiles_n = (p.N + 255) >> 8;
+  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int width = 4 * tiles_n, first = bid / width * 4, gsz = min(tiles_m - first, 4);
+  const int m0 = (first + bid % width % gsz) * 256, n0 = (bid % width / gsz) * 256;
+  const int left_m = min(p.M - 1 - m0, 255), left_n = min(p.N - 1 - n0, 255);
+  uint32_t ao[2][2], bo[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    n8_offsets<true>(p.lda, h, left_m, wid, lane, ao[h]);
+    n8_offsets<false>(p.ldb, h, left_n, wid, lane, bo[h]);
+  }
+  F8Trait<FA, FB> tr;
+  tr.begin(p, m0, n0, wid, lane);
+  f32x4_t acc[2][2][4][2];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  n8_loop(tr, lds, (const char*)p.A + (long)m0 * p.lda, (const char*)p.B + (long)n0 * p.ldb, tr.step(0), ao, bo, tr.nk2, wid,
+          lane, acc);
+  const bool fast = left_m == 255 && left_n == 255 && p.ldc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && p.ldaux % 8 == 0 &&
+                    (uintptr_t)p.aux % 16 == 0 && (uintptr_t)p.aux_out % 16 == 0;
+#pragma unroll
+  for (int qm = 0; qm < 2; ++qm)
+#pragma unroll
+    for (int qn = 0; qn < 2; ++qn)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[qm][qn][mt][e & 1][e >> 1];
+        f8_epi8<EPI, OutT>(p, fast, m0 + n8_row(wid, lane, qm, mt), n0 + n8_col(wid, lane, qn), v);
+      }
+}
+
 template <int EPI, typename OutT>
 static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s) {
   const long tiles = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
   if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles), block(256);
+  if constexpr (sizeof(OutT) == 2) {
+    const long big = (long)((p.M + 255) / 256) * ((p.N + 255) / 256);
+    if (p.nk > 0 && p.M >= 4 && p.N >= 2 && big >= 128) {
+      const dim3 g2((unsigned)big), b2(512);
+      if (fa == F8_E4M3 && fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E4M3, F8_E4M3>), g2, b2, 0, s, p);
+      else if (fa == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E4M3, F8_E5M2>), g2, b2, 0, s, p);
+      else if (fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E5M2, F8_E4M3>), g2, b2, 0, s, p);
+      else hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E5M2, F8_E5M2>), g2, b2, 0, s, p);
+      return hipGetLastError();
+    }
+  }
   if (fa == F8_E4M3 && fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E4M3, F8_E4M3>), grid, block, 0, s, p);
   else if (fa == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E4M3, F8_E5M2>), grid, block, 0, s, p);
   else if (fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E5M2, F8_E4M3>), grid, block, 0, s, p);

@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "nt8.h"
 
 namespace dllm {
 
@@ -260,9 +261,129 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_128(NsGemm p) {
     for (int k = 0; k < 4; ++k) ns_epi4<EPI>(p, z, m0 + wr * 64 + i * 16 + i15, n0 + wc * 64 + k * 16 + 4 * g, acc[i][k]);
 }
 
+// 256x256 tiles on the 8-phase loop (nt8.h): the three plane pairs as one run of 3 K / 64 K steps
+struct NsTrait {
+  const char *a, *b;
+  long pa, pb;          // bytes from the hi to the lo plane
+  int per;              // pairs of K steps per plane pair
+  int seg = 0, left;
+  __device__ __forceinline__ int advance(const char*& an, const char*& bn, int) {
+    if (--left > 0) {
+      an += 256;
+      bn += 256;
+    } else if (seg < 2) {   // (hi, lo) -> (lo, hi) -> (hi, hi)
+      an = a + (seg == 0 ? pa : 0);
+      bn = b;
+      ++seg;
+      left = per;
+    }
+    return 128;
+  }
+  template <class ODD> __device__ __forceinline__ void load(ODD, int) {}
+  template <int QM, int QN, int ODD>
+  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], const N8Frag (&fa)[4], const N8Frag (&fb)[2]) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+          c[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, s ? fb[nt].hi : fb[nt].lo),
+                                                             __builtin_bit_cast(f16x8_t, s ? fa[mt].hi : fa[mt].lo),
+                                                             c[mt][nt], 0, 0, 0);
+  }
+};
+
+// one row group of a lane: 8 columns n .. n + 7 of row m (v[e]), scaled and with the polynomial's other terms
+template <int EPI>
+__device__ __forceinline__ void ns_value8(const NsGemm& p, int z, int m, int n, float (&v)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= p.cs;
+  if constexpr (EPI == NS_POLY) {
+    const long o = (long)z * p.bo + (long)m * p.ldo + n;
+    const f16x8_t ah = *(const f16x8_t*)(p.aux + o), al = *(const f16x8_t*)(p.aux + p.po + o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      v[e] += p.cb * ((float)ah[e] + (float)al[e]) + (m == n + e ? p.ca : 0.f);
+  }
+}
+
+template <int EPI>
+__global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
+  __shared__ __attribute__((aligned(16))) char smem[N8_LDS];
+  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
+  const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
+  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int tiles_m = p.M >> 8, tiles_n = p.N >> 8;
+  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int width = 4 * tiles_n, first = bid / width * 4, gsz = min(tiles_m - first, 4);
+  const int m0 = (first + bid % width % gsz) * 256, n0 = (bid % width / gsz) * 256;
+  uint32_t ao[2][2], bo[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    n8_offsets<true>(p.lda * 2, h, 255, wid, lane, ao[h]);
+    n8_offsets<false>(p.ldb * 2, h, 255, wid, lane, bo[h]);
+  }
+  f32x4_t acc[2][2][4][2];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  NsTrait tr;
+  tr.a = (const char*)(p.A + (long)z * p.ba + (long)m0 * p.lda);
+  tr.b = (const char*)(p.B + (long)z * p.bb + (long)n0 * p.ldb);
+  tr.pa = p.pa * 2;
+  tr.pb = p.pb * 2;
+  tr.per = tr.left = p.K >> 7;
+  n8_loop(tr, lds, tr.a, tr.b + tr.pb, 128, ao, bo, 3 * (p.K >> 7), wid, lane, acc);
+
+#pragma unroll
+  for (int qm = 0; qm < 2; ++qm)
+#pragma unroll
+    for (int qn = 0; qn < 2; ++qn) {
+      const int n = n0 + n8_col(wid, lane, qn);
+      f16x4_t th[8], tl[8];   // transposed planes: column n + e, rows of the four mt
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const int m = m0 + n8_row(wid, lane, qm, mt);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[qm][qn][mt][e & 1][e >> 1];
+        if constexpr (EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY) {
+          ns_value8<EPI>(p, z, m, n, v);
+          f16x8_t h, l;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f16 hh, ll;
+            split16(v[e], hh, ll);
+            h[e] = hh;
+            l[e] = ll;
+            if constexpr (EPI == NS_PLANES_T) { th[e][mt] = hh; tl[e][mt] = ll; }
+          }
+          const long o = (long)z * p.bo + (long)m * p.ldo + n;
+          *(f16x8_t*)(p.out + o) = h;
+          *(f16x8_t*)(p.out + p.po + o) = l;
+        } else {
+          ns_epi4<EPI>(p, z, m, n, f32x4_t{v[0], v[1], v[2], v[3]});
+          ns_epi4<EPI>(p, z, m, n + 4, f32x4_t{v[4], v[5], v[6], v[7]});
+        }
+      }
+      if constexpr (EPI == NS_PLANES_T) {
+        const int m = m0 + n8_row(wid, lane, qm, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const long q = (long)z * p.bt + (long)(n + e) * p.ldt + m;
+          *(f16x4_t*)(p.outT + q) = th[e];
+          *(f16x4_t*)(p.outT + p.pt + q) = tl[e];
+        }
+      }
+    }
+}
+
 template <int EPI>
 static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
-  hipLaunchKernelGGL((ns_gemm_128<EPI>), dim3((p.M / 128) * (p.N / 128), B), dim3(256), 0, s, p);
+  if (p.M % 256 == 0 && p.N % 256 == 0)
+    hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3((p.M / 256) * (p.N / 256), B), dim3(512), 0, s, p);
+  else
+    hipLaunchKernelGGL((ns_gemm_128<EPI>), dim3((p.M / 128) * (p.N / 128), B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 

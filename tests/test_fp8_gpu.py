@@ -78,18 +78,18 @@ def product_check(got, qa, qb, alpha=1.0, beta=0.0, c=None, ref=None, mag_gain=1
     """|error| <= K u sum|a||b| (any order of fp32 accumulation, u = 2^-24) + half an output step.  bf16 results come from the
     8-bit matrix instruction, which aligns the products of 8 neighbouring k to the largest and drops what lies under 2^-13
     of it: at most 7 of the 8 lose less than 2^-13 of the largest each, so less than 7 * 2^-13 of the group's sum|a||b|."""
-    a, b = fp8.dequantize_fp8(qa).double().cpu(), fp8.dequantize_fp8(qb).double().cpu()
+    a, b = fp8.dequantize_fp8(qa).double().to(got.device), fp8.dequantize_fp8(qb).double().to(got.device)
     acc = a @ b.t()
     mag = abs(alpha) * (a.abs() @ b.abs().t())
     want = alpha * acc if ref is None else ref(acc)
     if beta:
-        want = want + beta * c.double().cpu()
-        mag = mag + abs(beta) * c.double().cpu().abs()
+        want = want + beta * c.double()
+        mag = mag + abs(beta) * c.double().abs()
     u = 2.0 ** -24
     half = torch.finfo(got.dtype).eps / 2
     unit = (qa.k + 2) * u + (7 * 2.0 ** -13 if got.dtype == torch.bfloat16 else 0.0)
     tol = mag_gain * unit * mag + half * want.abs() * (1 + half) + 1e-38
-    err = (got.double().cpu() - want).abs()
+    err = (got.double() - want).abs()
     assert (err <= tol).all(), f"worst {(err / tol).max().item():.3f} of the tolerance"
 
 
@@ -106,6 +106,27 @@ def test_gemm(M, N, K, fa, fb, out):
     product_check(fp8.gemm_fp8(qa, qb, c, alpha=0.75, beta=-0.5), qa, qb, 0.75, -0.5, c0)
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 33000, 300), (2817, 3001, 513), (33000, 5, 128), (4096, 2048, 256), (4, 32768, 640),
+                                   (2900, 3100, 1100)])
+@pytest.mark.parametrize("fa,fb", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_gemm_many_tiles(M, N, K, fa, fb, out):
+    """Grids that fill the chip: the large-tile kernels, odd and even numbers of K blocks, edges in both directions."""
+    qa, qb = fp8.quantize_fp8(rand(M, K, 1).to(DEV), fa), fp8.quantize_fp8(rand(N, K, 2).to(DEV), fb)
+    buf = torch.full((M + 1, N), 5.0, dtype=out, device=DEV)
+    product_check(fp8.gemm_fp8(qa, qb, buf[:M]), qa, qb)
+    assert (buf[M] == 5).all()
+    if fa == fb:
+        c0 = buf[:M].clone()
+        product_check(fp8.gemm_fp8(qa, qb, buf[:M], alpha=0.75, beta=-0.5), qa, qb, 0.75, -0.5, c0)
+        h = torch.empty(M, N, dtype=out, device=DEV)
+        a = fp8.gemm_fp8(qa, qb, out_dtype=out, epi="act", act="silu", aux_out=h)
+        product_check(h, qa, qb)
+        product_check(a, qa, qb, ref=lambda acc: act_fwd("silu", acc), mag_gain=1.13)
+        d = fp8.gemm_fp8(qa, qb, out_dtype=out, epi="dact", act="silu", aux=h)
+        product_check(d, qa, qb, ref=lambda acc: acc * act_grad("silu", h.double()), mag_gain=1.13)
+
+
 @pytest.mark.parametrize("M,N,K", [(3, 70, 200), (256, 512, 256), (300, 300, 513)])
 @pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
@@ -119,7 +140,7 @@ def test_gemm_activation_epilogues(M, N, K, act, out):
     same = fp8.gemm_fp8(qa, qb, out_dtype=out, epi="act", act=act)
     assert torch.equal(a, same)
     got = fp8.gemm_fp8(qa, qb, out_dtype=out, epi="dact", act=act, aux=h)
-    product_check(got, qa, qb, ref=lambda acc: acc * act_grad(act, h.double().cpu()), mag_gain=1.13)
+    product_check(got, qa, qb, ref=lambda acc: acc * act_grad(act, h.double()), mag_gain=1.13)
 
 
 def test_gemm_into_a_view_and_odd_strides():

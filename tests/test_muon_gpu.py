@@ -34,7 +34,7 @@ def tolerance(x, steps=5, dtype=torch.float32):
 
 
 SIZES = [(1, 1), (1, 200), (200, 1), (16, 16), (101, 300), (300, 101), (128, 128), (129, 257), (256, 512), (640, 384),
-         (64, 2000)]
+         (64, 2000), (512, 512), (700, 1500), (1500, 700)]
 
 
 @pytest.mark.parametrize("R,C", SIZES)
