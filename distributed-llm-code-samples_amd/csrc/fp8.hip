@@ -391,7 +391,22 @@ __global__ __launch_bounds__(256, 2) void fp8_gemm_128(Fp8GemmArgs p) {
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
 
-template <int FA, int FB>
+template <int FMT>
+__device__ __forceinline__ bf16x8_t codes8(int w0, int w1, float s) {
+  bf16x2_t v[4];
+  if constexpr (FMT == F8_E4M3) {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, false); v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, false); v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s, true);
+  } else {
+    v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w0, s, false); v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w0, s, true);
+    v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w1, s, false); v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w1, s, true);
+  }
+  return bf16x8_t{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
+}
+
+// EXACT: fp32 sums -- codes times scale as bf16 on the bf16 instruction (see codes_to_bf16), converted in the shadow of the
+// matrix instructions: 3 conversions (4 cycles each) per matrix instruction (16 cycles)
+template <int FA, int FB, bool EXACT>
 struct F8Trait {
   const uint8_t *sa, *sb;      // scale bytes of K step 0
   long ldsa, ldsb;
@@ -445,7 +460,7 @@ struct F8Trait {
     c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x, c, FB, FA, NT, b, MT, a);
   }
   template <int QM, int QN, int ODD>
-  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], const N8Frag (&fa)[4], const N8Frag (&fb)[2]) {
+  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], N8Frag (&fa)[4], N8Frag (&fb)[2]) {
     if constexpr (QM == 0 && QN == 0) {   // the step's first phase
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -455,6 +470,46 @@ struct F8Trait {
       }
     }
     const int a = wa[ODD][QM], b = wb[ODD][QN];
+    if constexpr (EXACT) {
+      // a fragment serves two phases; its conversion is repeated, not kept (32 more registers than there are)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(fa[i].lo), "+v"(fa[i].hi));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) asm volatile("" : "+v"(fb[i].lo), "+v"(fb[i].hi));
+      auto scale = [](int w, int i) { return __uint_as_float(((uint32_t)w >> (8 * i) & 255u) << 23); };
+      float sa4[4], sb2[2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sa4[i] = scale(a, i);
+      sb2[0] = scale(b, 0);
+      sb2[1] = scale(b, 1);
+      // quarter s of the fragments' codes (8 of 32); the next conversion is issued between a pair of matrix instructions
+      // and the order is pinned: left to itself the compiler converts everything first and spills
+      auto pick = [&](const N8Frag& f, int s, int k) { return s < 2 ? f.lo[2 * (s & 1) + k] : f.hi[2 * (s & 1) + k]; };
+      auto cva = [&](int s, int mt) { return codes8<FA>(pick(fa[mt], s, 0), pick(fa[mt], s, 1), sa4[mt]); };
+      auto cvb = [&](int s, int nt) { return codes8<FB>(pick(fb[nt], s, 0), pick(fb[nt], s, 1), sb2[nt]); };
+      bf16x8_t y0 = cvb(0, 0), y1 = cvb(0, 1), x = cva(0, 0), yn0 = y0, yn1 = y1;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          bf16x8_t xn = x;
+          c[mt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y0, x, c[mt][0], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (mt < 3) xn = cva(s, mt + 1);
+          else if (s < 3) xn = cva(s + 1, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          c[mt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y1, x, c[mt][1], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+          if (s < 3 && mt == 1) yn0 = cvb(s + 1, 0);
+          if (s < 3 && mt == 2) yn1 = cvb(s + 1, 1);
+          __builtin_amdgcn_sched_barrier(0);
+          x = xn;
+        }
+        y0 = yn0;
+        y1 = yn1;
+      }
+      return;
+    }
     one<0, 0>(c[0][0], fa[0], fb[0], a, b); one<0, 1>(c[0][1], fa[0], fb[1], a, b);
     one<1, 0>(c[1][0], fa[1], fb[0], a, b); one<1, 1>(c[1][1], fa[1], fb[1], a, b);
     one<2, 0>(c[2][0], fa[2], fb[0], a, b); one<2, 1>(c[2][1], fa[2], fb[1], a, b);
@@ -537,7 +592,7 @@ __global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
     n8_offsets<true>(p.lda, h, left_m, wid, lane, ao[h]);
     n8_offsets<false>(p.ldb, h, left_n, wid, lane, bo[h]);
   }
-  F8Trait<FA, FB> tr;
+  F8Trait<FA, FB, sizeof(OutT) == 4> tr;
   tr.begin(p, m0, n0, wid, lane);
   f32x4_t acc[2][2][4][2];
 #pragma unroll
@@ -564,7 +619,7 @@ static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s
   const long tiles = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
   if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
   const dim3 grid((unsigned)tiles), block(256);
-  if constexpr (sizeof(OutT) == 2) {
+  {
     const long big = (long)((p.M + 255) / 256) * ((p.N + 255) / 256);
     if (p.nk > 0 && p.M >= 4 && p.N >= 2 && big >= 128) {
       const dim3 g2((unsigned)big), b2(512);

@@ -281,7 +281,7 @@ struct NsTrait {
   }
   template <class ODD> __device__ __forceinline__ void load(ODD, int) {}
   template <int QM, int QN, int ODD>
-  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], const N8Frag (&fa)[4], const N8Frag (&fb)[2]) {
+  __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], N8Frag (&fa)[4], N8Frag (&fb)[2]) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll

@@ -121,7 +121,7 @@ __device__ __forceinline__ void n8_loop(T& t, DLLM_LDS char* lds, const char* a0
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
-  auto mma = [&](auto qm, auto qn, const N8Frag (&fb)[2], auto odd) {
+  auto mma = [&](auto qm, auto qn, N8Frag (&fb)[2], auto odd) {
     __builtin_amdgcn_s_setprio(1);
     t.template mma<qm.value, qn.value, odd.value>(acc[qm.value][qn.value], fa, fb);
     __builtin_amdgcn_s_setprio(0);
