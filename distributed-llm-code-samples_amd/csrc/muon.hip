@@ -34,7 +34,10 @@ constexpr int SX = 15, SA = 15, SP = 14, SQ = 10;   // plane scales 2^s of X, A 
 constexpr int NS_SEGMENT = 3;                        // steps on one Gram matrix where the result allows it
 constexpr int NS_PARTS = 256;                        // partial sums of squares per matrix
 
+// The empty asm makes v one fp32 number: where v is a product, the compiler otherwise rounds it to fp16 directly for one use
+// of h and by way of fp32 for another, and where the two differ hi + lo is off by a step of hi.
 __device__ __forceinline__ void split16(float v, f16& h, f16& l) {
+  asm("" : "+v"(v));
   h = (f16)v;
   l = (f16)(v - (float)h);
 }
@@ -61,28 +64,87 @@ __device__ __forceinline__ float muon_u(const MuonIn& p, long i) {
   return p.nesterov ? fmaf(p.beta, m, p.gscale * ld_g(p, i)) : m;
 }
 
+// four elements of g / the momentum at i (VEC: 16-byte aligned fp32, 8-byte aligned bf16; else one at a time)
+template <bool VEC>
+__device__ __forceinline__ f32x4_t ld_g4(const MuonIn& p, long i) {
+  if constexpr (!VEC) return f32x4_t{ld_g(p, i), ld_g(p, i + 1), ld_g(p, i + 2), ld_g(p, i + 3)};
+  if (p.gdt != DT_BF16) return *(const f32x4_t*)((const float*)p.g + i);
+  const uint2 w = *(const uint2*)((const uint16_t*)p.g + i);
+  return f32x4_t{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                 __uint_as_float(w.y & 0xffff0000u)};
+}
+template <int KIND, bool VEC>
+__device__ __forceinline__ f32x4_t muon_u4(const MuonIn& p, long i) {
+  if constexpr (KIND == NS_ORTH) return ld_g4<VEC>(p, i);
+  f32x4_t m;
+  if constexpr (VEC) m = *(const f32x4_t*)(p.mom + i);
+  else m = f32x4_t{p.mom[i], p.mom[i + 1], p.mom[i + 2], p.mom[i + 3]};
+  if (!p.nesterov) return m;
+  const f32x4_t g = ld_g4<VEC>(p, i);
+  f32x4_t u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) u[k] = fmaf(p.beta, m[k], p.gscale * g[k]);
+  return u;
+}
+
 // momentum update and the partial sums of u^2 (64-bit: gradients of any magnitude, and a sum that does not depend on how it
-// is cut).  grid (NS_PARTS, B)
-template <int KIND>
-__global__ __launch_bounds__(256) void muon_sumsq_kernel(MuonIn p, double* part) {
-  __shared__ double red[4];
-  const long n = (long)p.R * p.C, base = (long)blockIdx.y * n;
+// is cut).  grid (NS_PARTS, B).  Bound by HBM: one read of g (and of the momentum, and its write)
+template <int KIND, bool VEC>
+__device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, long base, long n) {
   double s = 0.0;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-    if constexpr (KIND == NS_MUON)
-      p.mom[base + i] = fmaf(p.beta, p.mom[base + i], p.gscale * ld_g(p, base + i));
-    const double u = (double)muon_u<KIND>(p, base + i);
+  const long n4 = VEC ? n >> 2 : 0, stride = (long)gridDim.x * blockDim.x, t0 = (long)blockIdx.x * blockDim.x + threadIdx.x;
+#pragma unroll 4
+  for (long j = t0; j < n4; j += stride) {
+    const long i = base + 4 * j;
+    if constexpr (KIND == NS_MUON) {
+      const f32x4_t g = ld_g4<VEC>(p, i);
+      f32x4_t m = *(const f32x4_t*)(p.mom + i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        m[k] = fmaf(p.beta, m[k], p.gscale * g[k]);
+        const double u = (double)(p.nesterov ? fmaf(p.beta, m[k], p.gscale * g[k]) : m[k]);
+        s += u * u;
+      }
+      *(f32x4_t*)(p.mom + i) = m;
+    } else {
+      const f32x4_t u = ld_g4<VEC>(p, i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s += (double)u[k] * (double)u[k];
+    }
+  }
+  for (long i = base + 4 * n4 + t0; i < base + n; i += stride) {
+    if constexpr (KIND == NS_MUON) p.mom[i] = fmaf(p.beta, p.mom[i], p.gscale * ld_g(p, i));
+    const double u = (double)muon_u<KIND>(p, i);
     s += u * u;
   }
+  return s;
+}
+// whether the matrix that starts at element `base` takes the 16-byte accesses
+template <int KIND>
+__device__ __forceinline__ bool muon_vec(const MuonIn& p, long base) {
+  const uintptr_t g = (uintptr_t)p.g + (uintptr_t)base * (p.gdt == DT_BF16 ? 2 : 4);
+  return g % 16 == 0 && (KIND == NS_ORTH || (uintptr_t)(p.mom + base) % 16 == 0);
+}
+
+template <int KIND>
+__global__ __launch_bounds__(1024) void muon_sumsq_kernel(MuonIn p, double* part) {
+  __shared__ double red[16];
+  const long n = (long)p.R * p.C, base = (long)blockIdx.y * n;
+  double s = muon_vec<KIND>(p, base) ? muon_sumsq_part<KIND, true>(p, base, n) : muon_sumsq_part<KIND, false>(p, base, n);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[(long)blockIdx.y * NS_PARTS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += red[i];
+    part[(long)blockIdx.y * NS_PARTS + blockIdx.x] = t;
+  }
 }
 
 // X0 planes in both orientations: same [Rp][Cp] and transposed [Cp][Rp], zeros outside [R][C].  64x64 tiles, grid
-// (Cp / 64, Rp / 64, B)
+// (Cp / 64, Rp / 64, B).  Bound by HBM: reads u once, writes four 2-byte planes
 template <int KIND>
 __global__ __launch_bounds__(256) void ns_split_kernel(MuonIn p, const double* part, float eps, f16* same, f16* tr, int Rp,
                                                        int Cp) {
@@ -99,24 +161,48 @@ __global__ __launch_bounds__(256) void ns_split_kernel(MuonIn p, const double* p
   const long plane = (long)Rp * Cp;
   f16* so = same + (long)blockIdx.z * 2 * plane;
   f16* to = tr + (long)blockIdx.z * 2 * plane;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  for (int k = t; k < 4096; k += 256) {
-    const int r = r0 + (k >> 6), c = c0 + (k & 63);
-    float v = 0.f;
-    if (r < p.R && c < p.C) v = muon_u<KIND>(p, ((long)blockIdx.z * p.R + r) * p.C + c) * inv;
-    tile[k >> 6][k & 63] = v;
-    f16 h, l;
-    split16(v, h, l);
-    so[(long)r * Cp + c] = h;
-    so[plane + (long)r * Cp + c] = l;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, q = t >> 4, j = 4 * (t & 15);
+  const bool vec = p.C % 8 == 0 && muon_vec<KIND>(p, (long)blockIdx.z * p.R * p.C);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = r0 + 16 * i + q, c = c0 + j;
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (r < p.R && c < p.C) {
+      const long o = ((long)blockIdx.z * p.R + r) * p.C + c;
+      if (vec) {
+        v = muon_u4<KIND, true>(p, o);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (c + k < p.C) v[k] = muon_u<KIND>(p, o + k);
+      }
+    }
+    f16x4_t h, l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f16 hh, ll;
+      split16(v[k] * inv, hh, ll);
+      h[k] = hh;
+      l[k] = ll;
+      tile[16 * i + q][j + k] = v[k] * inv;
+    }
+    *(f16x4_t*)(so + (long)r * Cp + c) = h;
+    *(f16x4_t*)(so + plane + (long)r * Cp + c) = l;
   }
   __syncthreads();
-  for (int k = t; k < 4096; k += 256) {
-    f16 h, l;
-    split16(tile[k & 63][k >> 6], h, l);
-    const long o = (long)(c0 + (k >> 6)) * Rp + r0 + (k & 63);
-    to[o] = h;
-    to[plane + o] = l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f16x4_t h, l;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f16 hh, ll;
+      split16(tile[j + k][16 * i + q], hh, ll);
+      h[k] = hh;
+      l[k] = ll;
+    }
+    const long o = (long)(c0 + 16 * i + q) * Rp + r0 + j;
+    *(f16x4_t*)(to + o) = h;
+    *(f16x4_t*)(to + plane + o) = l;
   }
 }
 
@@ -133,132 +219,75 @@ struct NsGemm {
   f16* out; long ldo, po, bo;          // planes (NS_PLANES / NS_PLANES_T / NS_POLY)
   f16* outT; long ldt, pt, bt;         // transposed planes (NS_PLANES_T)
   const f16* aux; float cb, ca;        // NS_POLY: A's planes (out's layout), b's factor, a on the diagonal
-  void* C; int cdt, R, Cc;             // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
+  void* C; int cdt, R, Cc, vec;        // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
   float* w; uint16_t* copy; int16_t* lo; float decay, rate;   // NS_STEP: fp32 master (+ bf16 copy), or split (lo, copy)
+  int sym;                             // the product is symmetric: tiles on and below the diagonal, mirrored on writing
 };
 
+// columns n .. n + 7 of row m of the result: written out (NS_OUT), or into the weights (NS_STEP)
 template <int EPI>
-__device__ __forceinline__ void ns_epi4(const NsGemm& p, int z, int m, int n, f32x4_t v) {
-  if constexpr (EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY) {
-    f16x4_t h, l;
-    const long o = (long)z * p.bo + (long)m * p.ldo + n;
-    f32x4_t a4 = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (EPI == NS_POLY) {
-      const f16x4_t ah = *(const f16x4_t*)(p.aux + o), al = *(const f16x4_t*)(p.aux + p.po + o);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) a4[r] = p.cb * ((float)ah[r] + (float)al[r]) + (m == n + r ? p.ca : 0.f);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      f16 hh, ll;
-      split16(EPI == NS_POLY ? fmaf(p.cs, v[r], a4[r]) : p.cs * v[r], hh, ll);
-      h[r] = hh;
-      l[r] = ll;
-    }
-    *(f16x4_t*)(p.out + o) = h;
-    *(f16x4_t*)(p.out + p.po + o) = l;
-    if constexpr (EPI == NS_PLANES_T) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const long q = (long)z * p.bt + (long)(n + r) * p.ldt + m;
-        p.outT[q] = h[r];
-        p.outT[p.pt + q] = l[r];
-      }
-    }
-  } else {
-    if (m >= p.R) return;
-    const long o = ((long)z * p.R + m) * p.Cc + n;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (n + r >= p.Cc) return;
-      const float x = p.cs * v[r];
-      if constexpr (EPI == NS_OUT) {
-        if (p.cdt == DT_BF16) ((uint16_t*)p.C)[o + r] = f2bf(x);
-        else ((float*)p.C)[o + r] = x;
-      } else if (p.lo != nullptr) {
-        const float w = split_join(p.copy[o + r], (uint16_t)p.lo[o + r]);
-        uint16_t h, l;
-        split_part(fmaf(-p.rate, x, w * p.decay), h, l);
-        p.copy[o + r] = h;
-        p.lo[o + r] = (int16_t)l;
+__device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n, const float (&v)[8]) {
+  if (m >= p.R || n >= p.Cc) return;
+  const long o = ((long)z * p.R + m) * p.Cc + n;
+  if (p.vec) {   // whole rows of 8, 16-byte aligned
+    if constexpr (EPI == NS_OUT) {
+      if (p.cdt == DT_BF16) {
+        uint4 u;
+        u.x = f2bf(p.cs * v[0]) | (uint32_t)f2bf(p.cs * v[1]) << 16; u.y = f2bf(p.cs * v[2]) | (uint32_t)f2bf(p.cs * v[3]) << 16;
+        u.z = f2bf(p.cs * v[4]) | (uint32_t)f2bf(p.cs * v[5]) << 16; u.w = f2bf(p.cs * v[6]) | (uint32_t)f2bf(p.cs * v[7]) << 16;
+        *(uint4*)((uint16_t*)p.C + o) = u;
       } else {
-        const float w = fmaf(-p.rate, x, p.w[o + r] * p.decay);
-        p.w[o + r] = w;
-        if (p.copy) p.copy[o + r] = f2bf(w);
+        *(f32x4_t*)((float*)p.C + o) = f32x4_t{p.cs * v[0], p.cs * v[1], p.cs * v[2], p.cs * v[3]};
+        *(f32x4_t*)((float*)p.C + o + 4) = f32x4_t{p.cs * v[4], p.cs * v[5], p.cs * v[6], p.cs * v[7]};
+      }
+    } else if (p.lo != nullptr) {
+      const uint4 wh = *(const uint4*)(p.copy + o), wl = *(const uint4*)((const uint16_t*)p.lo + o);
+      uint32_t h[4] = {wh.x, wh.y, wh.z, wh.w}, l[4] = {wl.x, wl.y, wl.z, wl.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float a, b;
+        split_join2(h[k], l[k], a, b);
+        split_part2(fmaf(-p.rate, p.cs * v[2 * k], a * p.decay), fmaf(-p.rate, p.cs * v[2 * k + 1], b * p.decay), h[k], l[k]);
+      }
+      *(uint4*)(p.copy + o) = uint4{h[0], h[1], h[2], h[3]};
+      *(uint4*)((uint16_t*)p.lo + o) = uint4{l[0], l[1], l[2], l[3]};
+    } else {
+      f32x4_t a = *(const f32x4_t*)(p.w + o), b = *(const f32x4_t*)(p.w + o + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        a[k] = fmaf(-p.rate, p.cs * v[k], a[k] * p.decay);
+        b[k] = fmaf(-p.rate, p.cs * v[4 + k], b[k] * p.decay);
+      }
+      *(f32x4_t*)(p.w + o) = a;
+      *(f32x4_t*)(p.w + o + 4) = b;
+      if (p.copy) {
+        uint4 u;
+        u.x = f2bf(a[0]) | (uint32_t)f2bf(a[1]) << 16; u.y = f2bf(a[2]) | (uint32_t)f2bf(a[3]) << 16;
+        u.z = f2bf(b[0]) | (uint32_t)f2bf(b[1]) << 16; u.w = f2bf(b[2]) | (uint32_t)f2bf(b[3]) << 16;
+        *(uint4*)(p.copy + o) = u;
       }
     }
+    return;
   }
-}
-
-// 128x128 tile, 4 waves of 64x64; K steps of 64 (one 128-byte line per row) over the three plane pairs (hi, lo), (lo, hi),
-// (hi, hi).  LDS rows of 128 B with XOR-swizzled 16-B chunks (conflict-free ds_read_b128), filled by LDS-DMA.
-template <int EPI>
-__global__ __launch_bounds__(256, 2) void ns_gemm_128(NsGemm p) {
-  constexpr int TB = 128 * 128;
-  __shared__ __attribute__((aligned(16))) char smem[4 * TB];
-  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
-  const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
-  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int tiles_n = p.N >> 7;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int m0 = (bid / tiles_n) * 128, n0 = (bid % tiles_n) * 128;
-  const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
-  const f16 *ap[4], *bp[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = i * 4 + wid, row = 8 * q + (lane >> 3), c = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
-    ap[i] = p.A + (long)z * p.ba + (long)(m0 + row) * p.lda + c;
-    bp[i] = p.B + (long)z * p.bb + (long)(n0 + row) * p.ldb + c;
-  }
-  const int nk = p.K >> 6;
-  // the small products first: the accumulator is rounded at its final size a third as often
-  auto stage = [&](int seg, int kt, int buf) {
-    DLLM_LDS char* d = lds + buf * 2 * TB;
-    const long oa = (long)kt * 64 + (seg == 1 ? p.pa : 0), ob = (long)kt * 64 + (seg == 0 ? p.pb : 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_global_load_lds((const DLLM_GLB void*)(ap[i] + oa), (DLLM_LDS void*)(d + (i * 4 + wid) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      __builtin_amdgcn_global_load_lds((const DLLM_GLB void*)(bp[i] + ob), (DLLM_LDS void*)(d + TB + (i * 4 + wid) * 1024), 16, 0, 0);
-  };
-  auto frag = [&](const DLLM_LDS char* tile, int row, int chunk) {
-    return *(const DLLM_LDS f16x8_t*)(tile + row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4));
-  };
-  f32x4_t acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[i][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  stage(0, 0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  int seg = 0, kt = 0;
-  for (int it = 0; it < 3 * nk; ++it) {
-    if (++kt == nk) { kt = 0; ++seg; }
-    if (it + 1 < 3 * nk) stage(seg, kt, (it + 1) & 1);
-    const DLLM_LDS char* As = lds + (it & 1) * 2 * TB;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      f16x8_t fa[4], fb[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        fa[i] = frag(As, wr * 64 + i * 16 + i15, 4 * s + g);
-        fb[i] = frag(As + TB, wc * 64 + i * 16 + i15, 4 * s + g);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[k], fa[i], acc[i][k], 0, 0, 0);
+  for (int r = 0; r < 8; ++r) {
+    if (n + r >= p.Cc) return;
+    const float x = p.cs * v[r];
+    if constexpr (EPI == NS_OUT) {
+      if (p.cdt == DT_BF16) ((uint16_t*)p.C)[o + r] = f2bf(x);
+      else ((float*)p.C)[o + r] = x;
+    } else if (p.lo != nullptr) {
+      const float w = split_join(p.copy[o + r], (uint16_t)p.lo[o + r]);
+      uint16_t h, l;
+      split_part(fmaf(-p.rate, x, w * p.decay), h, l);
+      p.copy[o + r] = h;
+      p.lo[o + r] = (int16_t)l;
+    } else {
+      const float w = fmaf(-p.rate, x, p.w[o + r] * p.decay);
+      p.w[o + r] = w;
+      if (p.copy) p.copy[o + r] = f2bf(w);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) ns_epi4<EPI>(p, z, m0 + wr * 64 + i * 16 + i15, n0 + wc * 64 + k * 16 + 4 * g, acc[i][k]);
 }
 
 // 256x256 tiles on the 8-phase loop (nt8.h): the three plane pairs as one run of 3 K / 64 K steps
@@ -308,16 +337,86 @@ __device__ __forceinline__ void ns_value8(const NsGemm& p, int z, int m, int n, 
   }
 }
 
+// tile `t` of a matrix -> its origin.  Symmetric products: row-wise over the lower triangle
+template <int TS>
+__device__ __forceinline__ void ns_tile(const NsGemm& p, int t, int& m0, int& n0) {
+  if (p.sym) {
+    int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+    while ((r + 1) * (r + 2) / 2 <= t) ++r;
+    while (r * (r + 1) / 2 > t) --r;
+    m0 = r * TS;
+    n0 = (t - r * (r + 1) / 2) * TS;
+    return;
+  }
+  const int tiles_m = (p.M + TS - 1) / TS, tiles_n = (p.N + TS - 1) / TS;
+  const int width = 4 * tiles_n, first = t / width * 4, gsz = min(tiles_m - first, 4);
+  m0 = (first + t % width % gsz) * TS;
+  n0 = (t % width / gsz) * TS;
+}
+static __host__ __device__ inline int ns_tiles(const NsGemm& p, int ts) {
+  const int a = (p.M + ts - 1) / ts, b = (p.N + ts - 1) / ts;
+  return p.sym ? a * (a + 1) / 2 : a * b;
+}
+
+// the tile's results from its accumulators
+template <int EPI>
+__device__ __forceinline__ void ns_finish(const NsGemm& p, int z, int m0, int n0, int wid, int lane,
+                                          const f32x4_t (&acc)[2][2][4][2]) {
+  constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
+  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
+  f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
+  const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
+#pragma unroll
+  for (int qm = 0; qm < 2; ++qm)
+#pragma unroll
+    for (int qn = 0; qn < 2; ++qn) {
+      const int n = n0 + n8_col(wid, lane, qn);
+      f16x4_t th[8], tl[8];   // transposed planes: column n + e, rows of the four mt
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const int m = m0 + n8_row(wid, lane, qm, mt);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[qm][qn][mt][e & 1][e >> 1];
+        if constexpr (PL) {
+          ns_value8<EPI>(p, z, m, n, v);
+          f16x8_t h, l;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f16 hh, ll;
+            split16(v[e], hh, ll);
+            h[e] = hh;
+            l[e] = ll;
+            th[e][mt] = hh;
+            tl[e][mt] = ll;
+          }
+          const long o = (long)z * p.bo + (long)m * p.ldo + n;
+          *(f16x8_t*)(p.out + o) = h;
+          *(f16x8_t*)(p.out + p.po + o) = l;
+        } else {
+          ns_result8<EPI>(p, z, m, n, v);
+        }
+      }
+      if (EPI == NS_PLANES_T || mirror) {
+        const int m = m0 + n8_row(wid, lane, qm, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const long q = (long)(n + e) * ldt + m;
+          *(f16x4_t*)(tp + q) = th[e];
+          *(f16x4_t*)(tp + pt + q) = tl[e];
+        }
+      }
+    }
+}
+
 template <int EPI>
 __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
   __shared__ __attribute__((aligned(16))) char smem[N8_LDS];
   DLLM_LDS char* lds = (DLLM_LDS char*)smem;
   const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
   const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int tiles_m = p.M >> 8, tiles_n = p.N >> 8;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int width = 4 * tiles_n, first = bid / width * 4, gsz = min(tiles_m - first, 4);
-  const int m0 = (first + bid % width % gsz) * 256, n0 = (bid % width / gsz) * 256;
+  int m0, n0;
+  ns_tile<256>(p, xcd_remap(blockIdx.x, gridDim.x), m0, n0);
   uint32_t ao[2][2], bo[2][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -334,56 +433,216 @@ __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
   tr.pb = p.pb * 2;
   tr.per = tr.left = p.K >> 7;
   n8_loop(tr, lds, tr.a, tr.b + tr.pb, 128, ao, bo, 3 * (p.K >> 7), wid, lane, acc);
+  ns_finish<EPI>(p, z, m0, n0, wid, lane, acc);
+}
+
+// ----------------------------------------------------------------------------------------------
+// 128x128 (F = 4) and 192x192 (F = 6) tiles: four waves, one per SIMD, each 16F x 16F
+//
+// For products whose 256x256 tiles do not fill the CUs: a symmetric 4096 x 4096 product has 136 of those and takes one
+// round on 256 CUs as the full 256 tiles do, but 253 of 192 x 192, one round of 0.56 of the work.
+// STAGES K steps of LDS ring, filled by LDS-DMA that many steps ahead; per K step one barrier.  A wave reads the fragments of
+// the next half step while it computes the current one; reads and fetches are placed between matrix instructions (order
+// pinned), so that the one wave of a SIMD keeps its matrix pipe busy.  Rows are permuted in LDS (slot 16 f + i holds row F i
+// + f of the wave's piece), so a lane ends with F consecutive rows by 4F consecutive columns.
+// ----------------------------------------------------------------------------------------------
+template <int F> struct W4 {
+  static constexpr int TS = 32 * F, OPB = TS * 128, STAGE = 2 * OPB;      // bytes of an operand's / a step's LDS
+  static constexpr int STAGES = F == 4 ? 4 : 3, PIECES = F;               // 1-KiB LDS-DMA pieces per wave and operand
+};
+
+template <int EPI, int F>
+__global__ __launch_bounds__(256, 1) void ns_gemm_w4(NsGemm p) {
+  using W = W4<F>;
+  __shared__ __attribute__((aligned(16))) char smem[W::STAGES * W::STAGE];
+  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
+  const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
+  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
+  int m0, n0;
+  ns_tile<W::TS>(p, xcd_remap(blockIdx.x, gridDim.x), m0, n0);
+  // a lane's byte offsets of its pieces (rows past the end re-load the last row: their results are not written)
+  uint32_t ao[F], bo[F];
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    const int s = 8 * (wid + 4 * i) + (lane >> 3);            // LDS slot 0 .. TS - 1
+    const int w = s / (16 * F), in = s - w * 16 * F;          // wave piece, slot in it
+    const int row = w * 16 * F + F * (in & 15) + (in >> 4), c = (lane & 7) ^ ((s >> 1) & 7);
+    ao[i] = (uint32_t)((long)min(row, p.M - 1 - m0) * p.lda * 2 + c * 16);
+    bo[i] = (uint32_t)((long)min(row, p.N - 1 - n0) * p.ldb * 2 + c * 16);
+  }
+  const char* A = (const char*)(p.A + (long)z * p.ba + (long)m0 * p.lda);
+  const char* B = (const char*)(p.B + (long)z * p.bb + (long)n0 * p.ldb);
+  const int per = p.K >> 6, nk = 3 * per;
+  // next step to fetch: (hi, lo), (lo, hi), (hi, hi); past the last one it stays there
+  const char *fa = A, *fb = B + p.pb * 2;
+  int fleft = per, fseg = 0;
+  auto next = [&]() {
+    if (--fleft > 0) {
+      fa += 128;
+      fb += 128;
+    } else if (fseg < 2) {
+      fa = A + (fseg == 0 ? p.pa * 2 : 0);
+      fb = B;
+      ++fseg;
+      fleft = per;
+    }
+  };
+  auto fetch_a = [&](int i, int slot) { n8_dma(fa, ao[i], lds + slot * W::STAGE + (wid + 4 * i) * 1024); };
+  auto fetch_b = [&](int i, int slot) { n8_dma(fb, bo[i], lds + slot * W::STAGE + W::OPB + (wid + 4 * i) * 1024); };
+  const uint32_t lb = (uint32_t)(uintptr_t)lds;
+  const int sw = (i15 >> 1) & 7;
+  const uint32_t ra[2] = {lb + (wr * 16 * F + i15) * 128 + ((g ^ sw) << 4), lb + (wr * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
+  const uint32_t rb[2] = {lb + W::OPB + (wc * 16 * F + i15) * 128 + ((g ^ sw) << 4),
+                          lb + W::OPB + (wc * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
+  n8_i32x4 xa[2][F], xb[2][F];      // [half step][fragment]
+  f32x4_t acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int k = 0; k < F; ++k) acc[i][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // read fragment j (0 .. 2F - 1: A's, then B's) of half step h from LDS slot address `off`
+  auto read = [&](auto h, auto j, uint32_t off) {
+    if constexpr (j.value < F) n8_read<j.value * 2048>(xa[h.value][j.value], ra[h.value] + off);
+    else n8_read<(j.value - F) * 2048>(xb[h.value][j.value - F], rb[h.value] + off);
+  };
+  auto mma1 = [&](int h, int q) {   // q-th of F * F
+    const int i = q / F, k = q % F;
+    acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, xb[h][k]),
+                                                       __builtin_bit_cast(f16x8_t, xa[h][i]), acc[i][k], 0, 0, 0);
+  };
+  auto each = [](auto f, auto... j) { (f(j), ...); };
+  auto for2f = [&](auto f) {
+    [&]<int... J>(std::integer_sequence<int, J...>) { each(f, std::integral_constant<int, J>{}...); }(std::make_integer_sequence<int, 2 * F>{});
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
 
 #pragma unroll
-  for (int qm = 0; qm < 2; ++qm)
+  for (int s = 0; s < W::STAGES - 1; ++s) {
 #pragma unroll
-    for (int qn = 0; qn < 2; ++qn) {
-      const int n = n0 + n8_col(wid, lane, qn);
-      f16x4_t th[8], tl[8];   // transposed planes: column n + e, rows of the four mt
+    for (int i = 0; i < F; ++i) fetch_a(i, s);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        const int m = m0 + n8_row(wid, lane, qm, mt);
+    for (int i = 0; i < F; ++i) fetch_b(i, s);
+    next();
+  }
+  // step 0 has landed when at most STAGES - 2 steps of 2F fetches are in flight
+  if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  N8_BARRIER();
+  for2f([&](auto j) { read(I0{}, j, 0u); });
+  N8_LDS_WAIT();
+  int slot = 0, fslot = W::STAGES - 1;   // LDS slots of the current step and of the next fetch
+  constexpr int PER = F * F / (2 * F);   // matrix instructions per read
+  for (int kt = 0; kt < nk; ++kt) {
+    const uint32_t off = (uint32_t)(slot * W::STAGE);
+    // first half: compute (kt, 0), read (kt, 1), fetch step kt + STAGES - 1 (its slot was last read in step kt - 1)
+    for2f([&](auto j) {
+      read(I1{}, j, off);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < PER; ++q) mma1(0, j.value * PER + q);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (j.value < F) fetch_a(j.value, fslot);
+      else fetch_b(j.value - F, fslot);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    next();
+    N8_LDS_WAIT();
+    // step kt + 1 has landed: at most STAGES - 2 younger steps in flight
+    if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    N8_BARRIER();
+    slot = slot + 1 == W::STAGES ? 0 : slot + 1;
+    fslot = fslot + 1 == W::STAGES ? 0 : fslot + 1;
+    const uint32_t offn = (uint32_t)(slot * W::STAGE);
+    // second half: compute (kt, 1), read (kt + 1, 0)
+    for2f([&](auto j) {
+      read(I0{}, j, offn);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < PER; ++q) mma1(1, j.value * PER + q);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    N8_LDS_WAIT();
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
+  constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
+  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
+  f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
+  const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
+  const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
+#pragma unroll
+  for (int c8 = 0; c8 < F / 2; ++c8) {            // 8 columns at a time
+    const int n = nb + 8 * c8;
+    if (n >= p.N) continue;
+    f16 th[8][F], tl[8][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int m = mb + i;
+      if (m < p.M) {
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[qm][qn][mt][e & 1][e >> 1];
-        if constexpr (EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY) {
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][(8 * c8 + e) % F][(8 * c8 + e) / F];
+        if constexpr (PL) {
           ns_value8<EPI>(p, z, m, n, v);
           f16x8_t h, l;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             f16 hh, ll;
             split16(v[e], hh, ll);
-            h[e] = hh;
-            l[e] = ll;
-            if constexpr (EPI == NS_PLANES_T) { th[e][mt] = hh; tl[e][mt] = ll; }
+            h[e] = hh; l[e] = ll;
+            th[e][i] = hh; tl[e][i] = ll;
           }
           const long o = (long)z * p.bo + (long)m * p.ldo + n;
           *(f16x8_t*)(p.out + o) = h;
           *(f16x8_t*)(p.out + p.po + o) = l;
         } else {
-          ns_epi4<EPI>(p, z, m, n, f32x4_t{v[0], v[1], v[2], v[3]});
-          ns_epi4<EPI>(p, z, m, n + 4, f32x4_t{v[4], v[5], v[6], v[7]});
-        }
-      }
-      if constexpr (EPI == NS_PLANES_T) {
-        const int m = m0 + n8_row(wid, lane, qm, 0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const long q = (long)z * p.bt + (long)(n + e) * p.ldt + m;
-          *(f16x4_t*)(p.outT + q) = th[e];
-          *(f16x4_t*)(p.outT + p.pt + q) = tl[e];
+          ns_result8<EPI>(p, z, m, n, v);
         }
       }
     }
+    if (EPI == NS_PLANES_T || mirror) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f16* o = tp + (long)(n + e) * ldt + mb;
+#pragma unroll
+        for (int i = 0; i < F; i += 2) {          // rows are even and M is a multiple of 128: pairs are inside or outside
+          if (mb + i < p.M) {
+            typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+            *(f16x2_t*)(o + i) = f16x2_t{th[e][i], th[e][i + 1]};
+            *(f16x2_t*)(o + pt + i) = f16x2_t{tl[e][i], tl[e][i + 1]};
+          }
+        }
+      }
+    }
+  }
+}
+
+static int ns_cus() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
+    return v;
+  }();
+  return n;
 }
 
 template <int EPI>
 static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
-  if (p.M % 256 == 0 && p.N % 256 == 0)
-    hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3((p.M / 256) * (p.N / 256), B), dim3(512), 0, s, p);
+  // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU
+  const long cus = ns_cus();
+  auto rounds = [&](int ts) { return (float)(((long)B * ns_tiles(p, ts) + cus - 1) / cus); };
+  const float t128 = rounds(128) * 0.35f, t192 = rounds(192) * 0.65f;
+  const float t256 = p.M % 256 == 0 && p.N % 256 == 0 ? rounds(256) * 1.5f : 1e30f;
+  if (t256 <= t128 && t256 <= t192)
+    hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3(ns_tiles(p, 256), B), dim3(512), 0, s, p);
+  else if (t192 < t128)
+    hipLaunchKernelGGL((ns_gemm_w4<EPI, 6>), dim3(ns_tiles(p, 192), B), dim3(256), 0, s, p);
   else
-    hipLaunchKernelGGL((ns_gemm_128<EPI>), dim3((p.M / 128) * (p.N / 128), B), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((ns_gemm_w4<EPI, 4>), dim3(ns_tiles(p, 128), B), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -430,7 +689,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
   NsSpace w = ns_space(ws, B, in.R, in.C, steps > seg);
   const int mp = (int)w.mp, np = (int)w.np;
   const int Rp = tall ? np : mp, Cp = tall ? mp : np;
-  hipLaunchKernelGGL((muon_sumsq_kernel<KIND>), dim3(NS_PARTS, B), dim3(256), 0, s, in, w.part);
+  hipLaunchKernelGGL((muon_sumsq_kernel<KIND>), dim3(NS_PARTS, B), dim3(1024), 0, s, in, w.part);
   NS_TRY(hipGetLastError());
   hipLaunchKernelGGL((ns_split_kernel<KIND>), dim3(Cp / 64, Rp / 64, B), dim3(256), 0, s, in, w.part, eps,
                      tall ? w.XT : w.X, tall ? w.X : w.XT, Rp, Cp);
@@ -443,6 +702,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
     p.B = b; p.ldb = mp; p.pb = psq; p.bb = w.sq;
     p.M = mp; p.N = mp; p.K = mp; p.cs = cs;
     p.out = out; p.ldo = mp; p.po = psq; p.bo = w.sq;
+    p.sym = 1;
     return p;
   };
   auto e2 = [](int e) { return e >= 0 ? (float)(1L << e) : 1.f / (float)(1L << -e); };
@@ -490,6 +750,8 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
       ap.B = b; ap.ldb = mp; ap.pb = tall ? psq : pbig; ap.bb = tall ? w.sq : w.big;
       ap.M = Rp; ap.N = Cp; ap.K = mp; ap.cs = e2(-sq - SX);
       ap.R = in.R; ap.Cc = in.C;
+      ap.vec = in.C % 8 == 0 && (uintptr_t)ap.C % 16 == 0 && (uintptr_t)ap.w % 16 == 0 && (uintptr_t)ap.copy % 16 == 0 &&
+               (uintptr_t)ap.lo % 16 == 0;
       NS_TRY(ns_launch<LAST>(ap, B, s));
     }
   }
