@@ -125,7 +125,9 @@ def check(rc: int, what: str) -> None:
 
 
 def stream_ptr(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle: 0.1 us, against 2 us for building the Stream object around it
+    idx = device.index if device is not None and device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(idx)
 
 
 DT = {torch.bfloat16: 0, torch.float32: 1}

@@ -337,21 +337,37 @@ __device__ __forceinline__ void ns_value8(const NsGemm& p, int z, int m, int n, 
   }
 }
 
-// tile `t` of a matrix -> its origin.  Symmetric products: row-wise over the lower triangle
+// The block's tile: matrix z and origin.  Blocks that run on one XCD (whose L2 they share) get consecutive tiles of all
+// matrices in a row, and consecutive tiles lie close together: bands of rows, column by column -- of the whole matrix, or
+// of its lower triangle (symmetric products).  32 tiles then need about 12 row panels, row by row they need 24 and the
+// products are bound by what lies behind the L2.
 template <int TS>
-__device__ __forceinline__ void ns_tile(const NsGemm& p, int t, int& m0, int& n0) {
-  if (p.sym) {
-    int r = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-    while ((r + 1) * (r + 2) / 2 <= t) ++r;
-    while (r * (r + 1) / 2 > t) --r;
-    m0 = r * TS;
-    n0 = (t - r * (r + 1) / 2) * TS;
+__device__ __forceinline__ void ns_tile(const NsGemm& p, int& z, int& m0, int& n0) {
+  const int tm = (p.M + TS - 1) / TS, tn = (p.N + TS - 1) / TS, nt = p.sym ? tm * (tm + 1) / 2 : tm * tn;
+  int t = xcd_remap(blockIdx.x, gridDim.x);
+  z = t / nt;
+  t -= z * nt;
+  constexpr int H = 6;
+  if (!p.sym) {
+    const int band = t / (H * tn), h = min(tm - band * H, H), in = t - band * H * tn;
+    m0 = (band * H + in % h) * TS;
+    n0 = in / h * TS;
     return;
   }
-  const int tiles_m = (p.M + TS - 1) / TS, tiles_n = (p.N + TS - 1) / TS;
-  const int width = 4 * tiles_n, first = t / width * 4, gsz = min(tiles_m - first, 4);
-  m0 = (first + t % width % gsz) * TS;
-  n0 = (t % width / gsz) * TS;
+  int r0 = 0;                                                    // first row of the band; r0 (r0 + 1) / 2 tiles before it
+  while (r0 + H < tm && (r0 + H) * (r0 + H + 1) / 2 <= t) r0 += H;
+  const int h = min(tm - r0, H);
+  t -= r0 * (r0 + 1) / 2;
+  int c = t / h, r = t - c * h;                                  // columns 0 .. r0 are h tiles high
+  if (c > r0) {                                                  // the triangle at the band's end
+    t -= (r0 + 1) * h;
+    c = 1;
+    while (t >= h - c) t -= h - c++;
+    r = c + t;
+    c += r0;
+  }
+  m0 = (r0 + r) * TS;
+  n0 = c * TS;
 }
 static __host__ __device__ inline int ns_tiles(const NsGemm& p, int ts) {
   const int a = (p.M + ts - 1) / ts, b = (p.N + ts - 1) / ts;
@@ -413,10 +429,10 @@ template <int EPI>
 __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
   __shared__ __attribute__((aligned(16))) char smem[N8_LDS];
   DLLM_LDS char* lds = (DLLM_LDS char*)smem;
-  const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63;
   const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
-  int m0, n0;
-  ns_tile<256>(p, xcd_remap(blockIdx.x, gridDim.x), m0, n0);
+  int z, m0, n0;
+  ns_tile<256>(p, z, m0, n0);
   uint32_t ao[2][2], bo[2][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -441,9 +457,9 @@ __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
 //
 // For products whose 256x256 tiles do not fill the CUs: a symmetric 4096 x 4096 product has 136 of those and takes one
 // round on 256 CUs as the full 256 tiles do, but 253 of 192 x 192, one round of 0.56 of the work.
-// STAGES K steps of LDS ring, filled by LDS-DMA that many steps ahead; per K step one barrier.  A wave reads the fragments of
-// the next half step while it computes the current one; reads and fetches are placed between matrix instructions (order
-// pinned), so that the one wave of a SIMD keeps its matrix pipe busy.  Rows are permuted in LDS (slot 16 f + i holds row F i
+// STAGES K steps of LDS ring, filled by LDS-DMA that many steps ahead; per K step one barrier.  A wave reads the next step's
+// fragments while it computes the current one's; reads and fetches are placed between matrix instructions (order pinned,
+// reads first so that they are back by the step's end), so that the one wave of a SIMD keeps its matrix pipe busy.  Rows are permuted in LDS (slot 16 f + i holds row F i
 // + f of the wave's piece), so a lane ends with F consecutive rows by 4F consecutive columns.
 // ----------------------------------------------------------------------------------------------
 template <int F> struct W4 {
@@ -456,11 +472,11 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_w4(NsGemm p) {
   using W = W4<F>;
   __shared__ __attribute__((aligned(16))) char smem[W::STAGES * W::STAGE];
   DLLM_LDS char* lds = (DLLM_LDS char*)smem;
-  const int t = threadIdx.x, lane = t & 63, z = blockIdx.y;
+  const int t = threadIdx.x, lane = t & 63;
   const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
   const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
-  int m0, n0;
-  ns_tile<W::TS>(p, xcd_remap(blockIdx.x, gridDim.x), m0, n0);
+  int z, m0, n0;
+  ns_tile<W::TS>(p, z, m0, n0);
   // a lane's byte offsets of its pieces (rows past the end re-load the last row: their results are not written)
   uint32_t ao[F], bo[F];
 #pragma unroll
@@ -495,76 +511,77 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_w4(NsGemm p) {
   const uint32_t ra[2] = {lb + (wr * 16 * F + i15) * 128 + ((g ^ sw) << 4), lb + (wr * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
   const uint32_t rb[2] = {lb + W::OPB + (wc * 16 * F + i15) * 128 + ((g ^ sw) << 4),
                           lb + W::OPB + (wc * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
-  n8_i32x4 xa[2][F], xb[2][F];      // [half step][fragment]
+  n8_i32x4 xa[2][2][F], xb[2][2][F];   // [step parity][half step][fragment]
   f32x4_t acc[F][F];
 #pragma unroll
   for (int i = 0; i < F; ++i)
 #pragma unroll
     for (int k = 0; k < F; ++k) acc[i][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // read fragment j (0 .. 2F - 1: A's, then B's) of half step h from LDS slot address `off`
-  auto read = [&](auto h, auto j, uint32_t off) {
-    if constexpr (j.value < F) n8_read<j.value * 2048>(xa[h.value][j.value], ra[h.value] + off);
-    else n8_read<(j.value - F) * 2048>(xb[h.value][j.value - F], rb[h.value] + off);
+  // read j of a step's 4F: half step 0's A and B fragments, then half step 1's
+  auto read = [&](auto par, auto j, uint32_t off) {
+    constexpr int h = j.value / (2 * F), f = j.value % (2 * F);
+    if constexpr (f < F) n8_read<f * 2048>(xa[par.value][h][f], ra[h] + off);
+    else n8_read<(f - F) * 2048>(xb[par.value][h][f - F], rb[h] + off);
   };
-  auto mma1 = [&](int h, int q) {   // q-th of F * F
-    const int i = q / F, k = q % F;
-    acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, xb[h][k]),
-                                                       __builtin_bit_cast(f16x8_t, xa[h][i]), acc[i][k], 0, 0, 0);
+  auto mma1 = [&](auto par, int q) {   // q-th of 2 F F
+    const int h = q / (F * F), i = q % (F * F) / F, k = q % F;
+    acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, xb[par.value][h][k]),
+                                                       __builtin_bit_cast(f16x8_t, xa[par.value][h][i]), acc[i][k], 0, 0, 0);
   };
-  auto each = [](auto f, auto... j) { (f(j), ...); };
-  auto for2f = [&](auto f) {
-    [&]<int... J>(std::integer_sequence<int, J...>) { each(f, std::integral_constant<int, J>{}...); }(std::make_integer_sequence<int, 2 * F>{});
+  auto upto = [](auto n, auto f) {
+    [&]<int... J>(std::integer_sequence<int, J...>) { (f(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, decltype(n)::value>{});
   };
   using I0 = std::integral_constant<int, 0>;
   using I1 = std::integral_constant<int, 1>;
+  using NR = std::integral_constant<int, 4 * F>;
+  using NF = std::integral_constant<int, 2 * F>;
 
 #pragma unroll
-  for (int s = 0; s < W::STAGES - 1; ++s) {
+  for (int s = 0; s < W::STAGES; ++s) {
 #pragma unroll
     for (int i = 0; i < F; ++i) fetch_a(i, s);
 #pragma unroll
     for (int i = 0; i < F; ++i) fetch_b(i, s);
     next();
   }
-  // step 0 has landed when at most STAGES - 2 steps of 2F fetches are in flight
-  if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  auto landed = [] {   // all but the youngest STAGES - 2 (2F fetches each) steps in flight have landed
+    if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  };
+  asm volatile("s_waitcnt vmcnt(24)" ::: "memory");   // (STAGES - 1) * 2F: step 0 has landed
   N8_BARRIER();
-  for2f([&](auto j) { read(I0{}, j, 0u); });
+  upto(NR{}, [&](auto j) { read(I0{}, j, 0u); });
   N8_LDS_WAIT();
-  int slot = 0, fslot = W::STAGES - 1;   // LDS slots of the current step and of the next fetch
-  constexpr int PER = F * F / (2 * F);   // matrix instructions per read
-  for (int kt = 0; kt < nk; ++kt) {
+  int slot = 0;
+  // step kt (fragments in registers, its LDS slot free): read step kt + 1, fetch step kt + STAGES into the freed slot
+  auto one = [&](auto par, auto other) {
+    landed();
+    N8_BARRIER();
+    const int fs = slot;
+    slot = slot + 1 == W::STAGES ? 0 : slot + 1;
     const uint32_t off = (uint32_t)(slot * W::STAGE);
-    // first half: compute (kt, 0), read (kt, 1), fetch step kt + STAGES - 1 (its slot was last read in step kt - 1)
-    for2f([&](auto j) {
-      read(I1{}, j, off);
+    constexpr int PR = F == 4 ? 1 : 2;             // matrix instructions per read, then two per fetch
+    upto(NR{}, [&](auto j) {
+      read(other, j, off);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int q = 0; q < PER; ++q) mma1(0, j.value * PER + q);
+      for (int q = 0; q < PR; ++q) mma1(par, j.value * PR + q);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (j.value < F) fetch_a(j.value, fslot);
-      else fetch_b(j.value - F, fslot);
+    });
+    upto(NF{}, [&](auto j) {
+      if constexpr (j.value < F) fetch_a(j.value, fs);
+      else fetch_b(j.value - F, fs);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) mma1(par, 4 * F * PR + j.value * 2 + q);
       __builtin_amdgcn_sched_barrier(0);
     });
     next();
     N8_LDS_WAIT();
-    // step kt + 1 has landed: at most STAGES - 2 younger steps in flight
-    if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-    N8_BARRIER();
-    slot = slot + 1 == W::STAGES ? 0 : slot + 1;
-    fslot = fslot + 1 == W::STAGES ? 0 : fslot + 1;
-    const uint32_t offn = (uint32_t)(slot * W::STAGE);
-    // second half: compute (kt, 1), read (kt + 1, 0)
-    for2f([&](auto j) {
-      read(I0{}, j, offn);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int q = 0; q < PER; ++q) mma1(1, j.value * PER + q);
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    N8_LDS_WAIT();
+  };
+  for (int kt = 0; kt < nk; kt += 2) {
+    one(I0{}, I1{});
+    one(I1{}, I0{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
@@ -632,17 +649,19 @@ static int ns_cus() {
 
 template <int EPI>
 static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
-  // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU
+  // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU (measured on full
+  // rounds: 128 x 128 is bound by LDS, the larger ones by the matrix units' power), and of a round's beginning and end
   const long cus = ns_cus();
-  auto rounds = [&](int ts) { return (float)(((long)B * ns_tiles(p, ts) + cus - 1) / cus); };
-  const float t128 = rounds(128) * 0.35f, t192 = rounds(192) * 0.65f;
-  const float t256 = p.M % 256 == 0 && p.N % 256 == 0 ? rounds(256) * 1.5f : 1e30f;
-  if (t256 <= t128 && t256 <= t192)
-    hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3(ns_tiles(p, 256), B), dim3(512), 0, s, p);
-  else if (t192 < t128)
-    hipLaunchKernelGGL((ns_gemm_w4<EPI, 6>), dim3(ns_tiles(p, 192), B), dim3(256), 0, s, p);
-  else
-    hipLaunchKernelGGL((ns_gemm_w4<EPI, 4>), dim3(ns_tiles(p, 128), B), dim3(256), 0, s, p);
+  const float steps = 3.f * (float)(p.K >> 6);
+  auto time = [&](int ts, float step) { return (float)(((long)B * ns_tiles(p, ts) + cus - 1) / cus) * (steps * step + 6.f); };
+  const float t128 = time(128, 0.40f), t192 = time(192, 0.75f);
+  const float t256 = p.M % 256 == 0 && p.N % 256 == 0 ? time(256, 1.5f) : 1e30f;
+  const int ts = t256 <= t128 && t256 <= t192 ? 256 : t192 < t128 ? 192 : 128;
+  const long grid = (long)B * ns_tiles(p, ts);
+  if (grid > 0x7fffffffL) return hipErrorInvalidValue;
+  if (ts == 256) hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3((unsigned)grid), dim3(512), 0, s, p);
+  else if (ts == 192) hipLaunchKernelGGL((ns_gemm_w4<EPI, 6>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((ns_gemm_w4<EPI, 4>), dim3((unsigned)grid), dim3(256), 0, s, p);
   return hipGetLastError();
 }
 
@@ -650,7 +669,8 @@ static long pad128(long n) { return (n + 127) / 128 * 128; }
 
 // workspace: partial sums, X and X^T planes (a second X^T when X is rewritten), six m x m plane pairs
 struct NsSpace {
-  long mp, np, big, sq;
+  long mp, np;              // sizes padded to 128
+  long px, ps;              // elements of an X (or X^T) and of an m x m plane
   double* part;
   f16 *X, *XT, *XT2, *S[6];
   size_t bytes;
@@ -659,8 +679,8 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
   NsSpace w;
   w.mp = pad128(min(R, C));
   w.np = pad128(max(R, C));
-  w.big = 2 * w.mp * w.np;
-  w.sq = 2 * w.mp * w.mp;
+  w.px = w.mp * w.np;
+  w.ps = w.mp * w.mp;
   size_t o = 0;
   auto take = [&](size_t n) {
     char* p = base + o;
@@ -668,10 +688,10 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
     return p;
   };
   w.part = (double*)take((size_t)B * NS_PARTS * 8);
-  w.X = (f16*)take((size_t)B * w.big * 2);
-  w.XT = (f16*)take((size_t)B * w.big * 2);
-  w.XT2 = again ? (f16*)take((size_t)B * w.big * 2) : nullptr;
-  for (int i = 0; i < 6; ++i) w.S[i] = (f16*)take((size_t)B * w.sq * 2);
+  w.X = (f16*)take((size_t)B * w.px * 4);
+  w.XT = (f16*)take((size_t)B * w.px * 4);
+  w.XT2 = again ? (f16*)take((size_t)B * w.px * 4) : nullptr;
+  for (int i = 0; i < 6; ++i) w.S[i] = (f16*)take((size_t)B * w.ps * 4);
   w.bytes = o;
   return w;
 }
@@ -695,13 +715,12 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
                      tall ? w.XT : w.X, tall ? w.X : w.XT, Rp, Cp);
   NS_TRY(hipGetLastError());
 
-  const long psq = w.sq / 2, pbig = w.big / 2;
   auto square = [&](const f16* a, const f16* b, f16* out, float cs) {   // [mp, mp] from two [mp, mp]
     NsGemm p = {};
-    p.A = a; p.lda = mp; p.pa = psq; p.ba = w.sq;
-    p.B = b; p.ldb = mp; p.pb = psq; p.bb = w.sq;
+    p.A = a; p.lda = mp; p.pa = w.ps; p.ba = 2 * w.ps;
+    p.B = b; p.ldb = mp; p.pb = w.ps; p.bb = 2 * w.ps;
     p.M = mp; p.N = mp; p.K = mp; p.cs = cs;
-    p.out = out; p.ldo = mp; p.po = psq; p.bo = w.sq;
+    p.out = out; p.ldo = mp; p.po = w.ps; p.bo = 2 * w.ps;
     p.sym = 1;
     return p;
   };
@@ -714,7 +733,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
     const int n = left > seg ? seg : left;
     left -= n;
     NsGemm gr = square(w.X, w.X, A, e2(SA - 2 * SX));
-    gr.lda = gr.ldb = np; gr.pa = gr.pb = pbig; gr.ba = gr.bb = w.big; gr.K = np;
+    gr.lda = gr.ldb = np; gr.pa = gr.pb = w.px; gr.ba = gr.bb = 2 * w.px; gr.K = np;
     NS_TRY(ns_launch<NS_PLANES>(gr, B, s));
     int sq = SP;
     for (int i = 0; i < n; ++i) {
@@ -736,18 +755,18 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
     NsGemm ap = {};
     const f16 *qa = Q, *xa = XT;
     if (left > 0) {   // X <- Q X and its transpose
-      ap.A = qa; ap.lda = mp; ap.pa = psq; ap.ba = w.sq;
-      ap.B = xa; ap.ldb = mp; ap.pb = pbig; ap.bb = w.big;
+      ap.A = qa; ap.lda = mp; ap.pa = w.ps; ap.ba = 2 * w.ps;
+      ap.B = xa; ap.ldb = mp; ap.pb = w.px; ap.bb = 2 * w.px;
       ap.M = mp; ap.N = np; ap.K = mp; ap.cs = e2(-sq);
-      ap.out = w.X; ap.ldo = np; ap.po = pbig; ap.bo = w.big;
-      ap.outT = XTn; ap.ldt = mp; ap.pt = pbig; ap.bt = w.big;
+      ap.out = w.X; ap.ldo = np; ap.po = w.px; ap.bo = 2 * w.px;
+      ap.outT = XTn; ap.ldt = mp; ap.pt = w.px; ap.bt = 2 * w.px;
       NS_TRY(ns_launch<NS_PLANES_T>(ap, B, s));
       f16* x = XT; XT = XTn; XTn = x;
     } else {          // the result, in U's own orientation
       ap = fin;
       const f16 *a = tall ? xa : qa, *b = tall ? qa : xa;
-      ap.A = a; ap.lda = mp; ap.pa = tall ? pbig : psq; ap.ba = tall ? w.big : w.sq;
-      ap.B = b; ap.ldb = mp; ap.pb = tall ? psq : pbig; ap.bb = tall ? w.sq : w.big;
+      ap.A = a; ap.lda = mp; ap.pa = tall ? w.px : w.ps; ap.ba = 2 * ap.pa;
+      ap.B = b; ap.ldb = mp; ap.pb = tall ? w.ps : w.px; ap.bb = 2 * ap.pb;
       ap.M = Rp; ap.N = Cp; ap.K = mp; ap.cs = e2(-sq - SX);
       ap.R = in.R; ap.Cc = in.C;
       ap.vec = in.C % 8 == 0 && (uintptr_t)ap.C % 16 == 0 && (uintptr_t)ap.w % 16 == 0 && (uintptr_t)ap.copy % 16 == 0 &&

@@ -58,11 +58,12 @@ def _fmt(fmt: str) -> torch.dtype:
     return FORMATS[fmt]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """Launches go to the tensors' device, whichever device is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def fp8_empty(rows: int, k: int, fmt: str = "e4m3", device=None) -> BlockFP8:
@@ -77,19 +78,21 @@ def _ld(t: torch.Tensor) -> int:
 
 
 def _check(q: BlockFP8, name: str) -> None:
-    if q.data.dim() != 2 or q.data.dtype not in _CODES:
-        raise TypeError(f"{name}: data must be a 2-D float8 tensor (e4m3fn or e5m2), got {q.data.dtype} {tuple(q.data.shape)}")
-    if q.k < 0 or q.data.shape[1] != _blocks(q.k) * BLOCK:
-        raise ValueError(f"{name}: data of k = {q.k} has {_blocks(q.k) * BLOCK} columns, got {q.data.shape[1]}")
-    if q.scale.dtype != torch.uint8 or tuple(q.scale.shape) != (_blocks(q.k), q.data.shape[0]):
-        raise ValueError(f"{name}: scale must be uint8 {(_blocks(q.k), q.data.shape[0])}, got {q.scale.dtype} "
-                         f"{tuple(q.scale.shape)}")
-    if q.scale.device != q.data.device:
-        raise ValueError(f"{name}: data on {q.data.device}, scale on {q.scale.device}")
-    if q.data.numel() and (q.data.stride(1) != 1 or (q.scale.stride(1) != 1 and q.scale.shape[1] > 1)):
-        raise ValueError(f"{name}: data and scale must be contiguous along their last dimension")
-    if q.data.device.type == "cuda" and q.data.numel() and (q.data.data_ptr() % 16 or _ld(q.data) % 16):
-        raise ValueError(f"{name}: data rows must start at multiples of 16 bytes")
+    d, sc, k = q
+    if d.dtype not in _CODES or d.dim() != 2:
+        raise TypeError(f"{name}: data must be a 2-D float8 tensor (e4m3fn or e5m2), got {d.dtype} {tuple(d.shape)}")
+    rows, cols = d.shape
+    if k < 0 or cols != -(-k // BLOCK) * BLOCK:
+        raise ValueError(f"{name}: data of k = {k} has {_blocks(k) * BLOCK} columns, got {cols}")
+    if sc.dtype != torch.uint8 or sc.shape != (cols // BLOCK, rows):
+        raise ValueError(f"{name}: scale must be uint8 {(_blocks(k), rows)}, got {sc.dtype} {tuple(sc.shape)}")
+    if sc.device != d.device:
+        raise ValueError(f"{name}: data on {d.device}, scale on {sc.device}")
+    if rows and cols:
+        if d.stride(1) != 1 or (rows > 1 and sc.stride(1) != 1):
+            raise ValueError(f"{name}: data and scale must be contiguous along their last dimension")
+        if d.is_cuda and (d.data_ptr() % 16 or _ld(d) % 16):
+            raise ValueError(f"{name}: data rows must start at multiples of 16 bytes")
 
 
 def _pow2(e: torch.Tensor) -> torch.Tensor:
@@ -114,48 +117,56 @@ def _quantize_torch(x: torch.Tensor, dt: torch.dtype, tile: bool, out: BlockFP8)
     out.scale.copy_((e + 127).to(torch.uint8).expand(v.shape[0], v.shape[1], kb, 1).reshape(-1, kb)[:R].t())
 
 
-def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bool) -> None:
+def _check_out(o: BlockFP8, rows: int, k: int, device, name: str) -> BlockFP8:
+    _check(o, name)
+    if o.rows != rows or o.k != k or o.device != device:
+        raise ValueError(f"{name} must hold {(rows, k)} on {device}, got {(o.rows, o.k)} on {o.device}")
+    return o
+
+
+def _shape2(x: torch.Tensor) -> tuple[int, int]:
     if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
+    return x.shape
+
+
+def _arg(o: BlockFP8 | None) -> tuple:
+    return (None, 0, None, 0) if o is None else (o.data.data_ptr(), _ld(o.data), o.scale.data_ptr(), _ld(o.scale))
+
+
+def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bool) -> None:
     R, C = x.shape
-    for o, rows, k, name in ((q, R, C, "out"), (qt, C, R, "out_t")):
-        if o is None:
-            continue
-        _check(o, name)
-        if o.rows != rows or o.k != k or o.device != x.device:
-            raise ValueError(f"{name} must hold {(rows, k)} on {x.device}, got {(o.rows, o.k)} on {o.device}")
     if R == 0 or C == 0:
         return
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         if q is not None:
             _quantize_torch(x, q.data.dtype, tile, q)
         if qt is not None:
             _quantize_torch(x.t(), qt.data.dtype, tile, qt)
         return
-    if x.stride(1) != 1 and C > 1:
+    if C > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    null = (None, 0, None, 0)
-    arg = lambda o: null if o is None else (o.data.data_ptr(), _ld(o.data), o.scale.data_ptr(),  # noqa: E731
-                                            _ld(o.scale))
-    code = lambda o: 0 if o is None else _CODES[o.data.dtype]  # noqa: E731
     with _on(x.device):
-        rc = _native.lib().dllm_fp8_quantize(x.data_ptr(), _native.dtype_code(x.dtype), x.stride(0), R, C, *arg(q), *arg(qt),
-                                             code(q), code(qt), int(tile), _native.stream_ptr(x.device))
-    _native.check(rc, f"dllm_fp8_quantize({R}x{C})")
+        rc = _native.lib().dllm_fp8_quantize(x.data_ptr(), _native.DT[x.dtype], x.stride(0), R, C, *_arg(q), *_arg(qt),
+                                             _CODES[q.data.dtype] if q is not None else 0,
+                                             _CODES[qt.data.dtype] if qt is not None else 0, int(tile),
+                                             _native.stream_ptr(x.device))
+    if rc:
+        _native.check(rc, f"dllm_fp8_quantize({R}x{C})")
 
 
 def quantize_fp8(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
     """The 8-bit form of ``x`` [R, K] (bf16 / fp32), scaled per row and 128 columns (``tile``: per 128x128 tile)."""
-    if out is None:
-        out = fp8_empty(*_shape2(x), fmt, x.device)
+    R, C = _shape2(x)
+    out = fp8_empty(R, C, fmt, x.device) if out is None else _check_out(out, R, C, x.device, "out")
     _quantize(x, out, None, tile)
     return out
 
 
 def quantize_fp8_t(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
     """The 8-bit form of ``xᵀ`` [K, R], scaled per column of ``x`` and 128 rows (``tile``: per 128x128 tile)."""
-    if out is None:
-        out = fp8_empty(*reversed(_shape2(x)), fmt, x.device)
+    R, C = _shape2(x)
+    out = fp8_empty(C, R, fmt, x.device) if out is None else _check_out(out, C, R, x.device, "out")
     _quantize(x, None, out, tile)
     return out
 
@@ -165,16 +176,10 @@ def quantize_fp8_both(x: torch.Tensor, fmt: str = "e4m3", fmt_t: str = "e4m3", *
     """``(quantize_fp8(x, fmt), quantize_fp8_t(x, fmt_t))`` from one read of ``x``: a forward (or input-gradient) operand
     and the weight-gradient operand of the same tensor."""
     R, C = _shape2(x)
-    out = fp8_empty(R, C, fmt, x.device) if out is None else out
-    out_t = fp8_empty(C, R, fmt_t, x.device) if out_t is None else out_t
+    out = fp8_empty(R, C, fmt, x.device) if out is None else _check_out(out, R, C, x.device, "out")
+    out_t = fp8_empty(C, R, fmt_t, x.device) if out_t is None else _check_out(out_t, C, R, x.device, "out_t")
     _quantize(x, out, out_t, tile)
     return out, out_t
-
-
-def _shape2(x: torch.Tensor) -> tuple[int, int]:
-    if x.dim() != 2:
-        raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
-    return x.shape[0], x.shape[1]
 
 
 def dequantize_fp8(q: BlockFP8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
