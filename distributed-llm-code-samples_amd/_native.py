@@ -60,7 +60,8 @@ _SIGS = {
                                     c_void_p]),
     "dllm_fp8_gemm": (c_int, [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_long, c_void_p, c_long, c_int,
                               c_void_p, c_long, c_int, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_float,
-                              c_int, c_int, c_void_p]),
+                              c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
+    "dllm_fp8_gemm_plan": (c_int, [c_int, c_int, c_int, c_int]),
     "dllm_muon_workspace": (c_long, [c_int, c_int, c_int, c_int]),
     "dllm_orthogonalize": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_long,
                                    c_void_p]),

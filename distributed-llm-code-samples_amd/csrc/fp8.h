@@ -40,6 +40,8 @@ struct Fp8GemmArgs {
   int M, N, nk;            // nk: 128-deep K steps
   float alpha, beta;
   int act;
+  int tile, ksplit;        // output tile; K slices (fp32 sums of slice s at ws + s M N)
+  float* ws;
 };
 
 }  // namespace dllm

@@ -213,18 +213,14 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* q, l
 }
 
 // ----------------------------------------------------------------------------------------------
-// product C = alpha A B^T + beta C (and the activation epilogues), any M, N: 128x128 tile, 4 waves of 64x64
+// product C = alpha A B^T + beta C (and the activation epilogues), any M, N
 //
-// Both operands are K-contiguous; a K step is one 128-byte line per row.  LDS rows of 128 B with the 16-B chunk index
-// XOR-swizzled by (row >> 1) & 7, filled by LDS-DMA from swizzled source addresses and read by ds_read_b128 without bank
-// conflicts.  A lane's 32 bytes of a fragment are chunks g and 4 + g (g = lane / 16) of its row, in A and B alike: a
-// permutation of k inside the block, which the sum and the block's one scale do not see.  The operands are swapped in
-// the matrix instruction (B first), so a lane ends with 4 consecutive columns of one row of C.
+// Both operands are K-contiguous; a K step of 128 is one 128-byte line per row.  A lane's 32 bytes of a fragment are 16-byte
+// chunks g and 4 + g (g = lane / 16) of its row, in A and B alike: a permutation of k inside the block, which neither the
+// sum nor the block's one scale sees.  The operands are swapped in the matrix instruction (B first), so a lane ends with
+// consecutive columns of a row of C.  Three kernels: 256x256 tiles (8-phase loop), 128x128 and 64x64 tiles (one wave per
+// quarter), and few rows or columns (operands straight to registers, K over the waves); dllm_fp8_gemm picks.
 // ----------------------------------------------------------------------------------------------
-__device__ __forceinline__ void lds_dma16(const uint8_t* src, DLLM_LDS char* dst) {
-  __builtin_amdgcn_global_load_lds((const DLLM_GLB void*)src, (DLLM_LDS void*)dst, 16, 0, 0);
-}
-
 template <int FB, int FA>
 __device__ __forceinline__ f32x4_t mfma_f8(i32x8_t b, i32x8_t a, f32x4_t c, int sb, int sa) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, FB, FA, 0, sb, 0, sa);
@@ -236,161 +232,6 @@ __device__ __forceinline__ f32x4_t mfma_f8(i32x8_t b, i32x8_t a, f32x4_t c, int 
 // the bf16 instruction, which keeps fp32 sums (5e-7 at K = 8192): codes times their scale are bf16 numbers, exactly
 // (8 exponent bits; only values under 2^-126 may round), so the operands convert in registers on their way from LDS.
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
-template <int FMT>
-__device__ __forceinline__ void codes_to_bf16(i32x8_t q, float s, bf16x8_t (&o)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    bf16x2_t v[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int w = q[2 * i + h];
-      if constexpr (FMT == F8_E4M3) {
-        v[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false);
-        v[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true);
-      } else {
-        v[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, false);
-        v[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, true);
-      }
-    }
-    o[i] = bf16x8_t{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
-  }
-}
-
-template <typename OutT> __device__ __forceinline__ float ld_out(const void* p, long i) {
-  if constexpr (sizeof(OutT) == 2) return bf2f(((const uint16_t*)p)[i]);
-  else return ((const float*)p)[i];
-}
-template <typename OutT> __device__ __forceinline__ void st_out(void* p, long i, float v) {
-  if constexpr (sizeof(OutT) == 2) ((uint16_t*)p)[i] = f2bf(v);
-  else ((float*)p)[i] = v;
-}
-
-// epilogue of 4 consecutive columns n .. n+3 of row m
-template <int EPI, typename OutT>
-__device__ __forceinline__ void f8_epi4(const Fp8GemmArgs& p, int m, int n, f32x4_t v) {
-  if (m >= p.M) return;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (n + r >= p.N) return;
-    const long i = (long)m * p.ldc + n + r, ia = (long)m * p.ldaux + n + r;
-    float o = v[r];
-    if constexpr (EPI == EPI_STORE) {
-      o *= p.alpha;
-      if (p.beta != 0.f) o += p.beta * ld_out<OutT>(p.C, i);
-    } else if constexpr (EPI == EPI_ACT) {
-      if (p.aux_out) st_out<OutT>(p.aux_out, ia, o);
-      o = act_fwd(p.act, o);
-    } else {
-      o *= act_grad(p.act, ld_out<OutT>(p.aux, ia));
-    }
-    st_out<OutT>(p.C, i, o);
-  }
-}
-
-template <int EPI, typename OutT, int FA, int FB>
-__global__ __launch_bounds__(256, 2) void fp8_gemm_128(Fp8GemmArgs p) {
-  constexpr int TB = 128 * 128;
-  __shared__ __attribute__((aligned(16))) char smem[4 * TB];   // [buffer][A, B]
-  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
-  const int t = threadIdx.x, lane = t & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int tiles_n = (p.N + 127) >> 7;
-  const int bid = xcd_remap(blockIdx.x, gridDim.x);
-  const int m0 = (bid / tiles_n) * 128, n0 = (bid % tiles_n) * 128;
-  const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
-
-  // rows past the end re-load the last row: their products are never stored
-  const uint8_t *ap[4], *bp[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int q = i * 4 + wid, row = 8 * q + (lane >> 3), c = ((lane & 7) ^ ((row >> 1) & 7)) * 16;
-    ap[i] = p.A + (long)min(m0 + row, p.M - 1) * p.lda + c;
-    bp[i] = p.B + (long)min(n0 + row, p.N - 1) * p.ldb + c;
-  }
-  auto stage = [&](int kt, int buf) {
-    DLLM_LDS char* d = lds + buf * 2 * TB;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lds_dma16(ap[i] + (long)kt * 128, d + (i * 4 + wid) * 1024);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) lds_dma16(bp[i] + (long)kt * 128, d + TB + (i * 4 + wid) * 1024);
-  };
-  auto frag = [&](const DLLM_LDS char* tile, int row) {
-    const int f = (row >> 1) & 7;
-    const i32x4_t lo = *(const DLLM_LDS i32x4_t*)(tile + row * 128 + ((g ^ f) << 4));
-    const i32x4_t hi = *(const DLLM_LDS i32x4_t*)(tile + row * 128 + (((4 + g) ^ f) << 4));
-    return i32x8_t{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  };
-  int am[4], bn[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    am[i] = min(m0 + wr * 64 + i * 16 + i15, p.M - 1);
-    bn[i] = min(n0 + wc * 64 + i * 16 + i15, p.N - 1);
-  }
-
-  f32x4_t acc[4][4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[i][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  if (p.nk > 0) stage(0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  for (int kt = 0; kt < p.nk; ++kt) {
-    if (kt + 1 < p.nk) stage(kt + 1, (kt + 1) & 1);
-    const DLLM_LDS char* As = lds + (kt & 1) * 2 * TB;
-    int sa[4], sb[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sa[i] = p.SA[(long)kt * p.ldsa + am[i]];
-      sb[i] = p.SB[(long)kt * p.ldsb + bn[i]];
-    }
-    i32x8_t fa[4], fb[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      fa[i] = frag(As, wr * 64 + i * 16 + i15);
-      fb[i] = frag(As + TB, wc * 64 + i * 16 + i15);
-    }
-    if constexpr (sizeof(OutT) == 2) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[i][k] = mfma_f8<FB, FA>(fb[k], fa[i], acc[i][k], sb[k], sa[i]);
-    } else {
-      bf16x8_t xb[4][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) codes_to_bf16<FB>(fb[k], e8m0_to_f32(sb[k]), xb[k]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bf16x8_t xa[4];
-        codes_to_bf16<FA>(fa[i], e8m0_to_f32(sa[i]), xa);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb[k][q], xa[q], acc[i][k], 0, 0, 0);
-      }
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      f8_epi4<EPI, OutT>(p, m0 + wr * 64 + i * 16 + i15, n0 + wc * 64 + k * 16 + 4 * g, acc[i][k]);
-}
-
-// ----------------------------------------------------------------------------------------------
-// 256x256 tiles on the 8-phase loop (nt8.h), one matrix instruction per 16x16 fragment pair and K step.
-//
-// Scales: a lane's four A rows of a half are consecutive rows of C (nt8.h), so one 32-bit word of the K step's scale row
-// holds them, and 16 bits its two B rows; the matrix instruction picks the byte (op_sel), so scaling costs two 4-byte and
-// two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more: the last step again, with scale
-// bytes 0 on both sides, 2^-254 of it, which leaves every fp32 sum as it is.
-// ----------------------------------------------------------------------------------------------
-typedef uint32_t u32_any __attribute__((aligned(1)));
-typedef uint16_t u16_any __attribute__((aligned(1)));
-
 template <int FMT>
 __device__ __forceinline__ bf16x8_t codes8(int w0, int w1, float s) {
   bf16x2_t v[4];
@@ -404,7 +245,49 @@ __device__ __forceinline__ bf16x8_t codes8(int w0, int w1, float s) {
   return bf16x8_t{v[0][0], v[0][1], v[1][0], v[1][1], v[2][0], v[2][1], v[3][0], v[3][1]};
 }
 
-// EXACT: fp32 sums -- codes times scale as bf16 on the bf16 instruction (see codes_to_bf16), converted in the shadow of the
+template <typename OutT> __device__ __forceinline__ float ld_out(const void* p, long i) {
+  if constexpr (sizeof(OutT) == 2) return bf2f(((const uint16_t*)p)[i]);
+  else return ((const float*)p)[i];
+}
+template <typename OutT> __device__ __forceinline__ void st_out(void* p, long i, float v) {
+  if constexpr (sizeof(OutT) == 2) ((uint16_t*)p)[i] = f2bf(v);
+  else ((float*)p)[i] = v;
+}
+
+// epilogue of element (m, n)
+template <int EPI, typename OutT>
+__device__ __forceinline__ void f8_epi1(const Fp8GemmArgs& p, int m, int n, float o) {
+  const long i = (long)m * p.ldc + n, ia = (long)m * p.ldaux + n;
+  if constexpr (EPI == EPI_STORE) {
+    o *= p.alpha;
+    if (p.beta != 0.f) o += p.beta * ld_out<OutT>(p.C, i);
+  } else if constexpr (EPI == EPI_ACT) {
+    if (p.aux_out) st_out<OutT>(p.aux_out, ia, o);
+    o = act_fwd(p.act, o);
+  } else {
+    o *= act_grad(p.act, ld_out<OutT>(p.aux, ia));
+  }
+  st_out<OutT>(p.C, i, o);
+}
+// whether rows of C and aux take 16-byte accesses
+template <typename OutT>
+__device__ __forceinline__ bool f8_aligned(const Fp8GemmArgs& p) {
+  return p.ldc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && p.ldaux % 8 == 0 && (uintptr_t)p.aux % 16 == 0 &&
+         (uintptr_t)p.aux_out % 16 == 0;
+}
+
+// ----------------------------------------------------------------------------------------------
+// 256x256 tiles on the 8-phase loop (nt8.h), one matrix instruction per 16x16 fragment pair and K step.
+//
+// Scales: a lane's four A rows of a half are consecutive rows of C (nt8.h), so one 32-bit word of the K step's scale row
+// holds them, and 16 bits its two B rows; the matrix instruction picks the byte (op_sel), so scaling costs two 4-byte and
+// two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more: the last step again, with scale
+// bytes 0 on both sides, 2^-254 of it, which leaves every fp32 sum as it is.
+// ----------------------------------------------------------------------------------------------
+typedef uint32_t u32_any __attribute__((aligned(1)));
+typedef uint16_t u16_any __attribute__((aligned(1)));
+
+// EXACT: fp32 sums -- codes times scale as bf16 on the bf16 instruction (see codes8), converted in the shadow of the
 // matrix instructions: 3 conversions (4 cycles each) per matrix instruction (16 cycles)
 template <int FA, int FB, bool EXACT>
 struct F8Trait {
@@ -521,8 +404,10 @@ struct F8Trait {
 template <int EPI, typename OutT>
 __device__ __forceinline__ void f8_epi8(const Fp8GemmArgs& p, bool fast, int m, int n, const float (&v)[8]) {
   if (!fast) {
-    f8_epi4<EPI, OutT>(p, m, n, f32x4_t{v[0], v[1], v[2], v[3]});
-    f8_epi4<EPI, OutT>(p, m, n + 4, f32x4_t{v[4], v[5], v[6], v[7]});
+    if (m < p.M)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < p.N) f8_epi1<EPI, OutT>(p, m, n + e, v[e]);
     return;
   }
   auto load = [](const void* base, long i, float (&x)[8]) {
@@ -599,8 +484,7 @@ __global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
   for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   n8_loop(tr, lds, (const char*)p.A + (long)m0 * p.lda, (const char*)p.B + (long)n0 * p.ldb, tr.step(0), ao, bo, tr.nk2, wid,
           lane, acc);
-  const bool fast = left_m == 255 && left_n == 255 && p.ldc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && p.ldaux % 8 == 0 &&
-                    (uintptr_t)p.aux % 16 == 0 && (uintptr_t)p.aux_out % 16 == 0;
+  const bool fast = left_m == 255 && left_n == 255 && f8_aligned<OutT>(p);
 #pragma unroll
   for (int qm = 0; qm < 2; ++qm)
 #pragma unroll
@@ -614,27 +498,330 @@ __global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
       }
 }
 
+// ----------------------------------------------------------------------------------------------
+// 128x128 (F = 4) and 64x64 (F = 2) tiles: four waves, each 16F x 16F, a ring of 4 K steps of LDS
+//
+// For grids that 256x256 tiles leave part-empty.  A wave reads the next step's fragments while it computes the current
+// step's; one barrier per step.  F = 4 is bound by LDS (64 KiB read and 32 KiB written per step, 768 of its about 830
+// cycles), F = 2 by the latency of few steps.  Rows are permuted in LDS (slot 16 f + i holds row F i + f of the wave's
+// piece): a lane's F rows are consecutive and one word holds their scales.  ksplit > 1: slice blockIdx.y of the K steps,
+// fp32 partial sums to ws (fp8_join adds them).
+// ----------------------------------------------------------------------------------------------
+template <int EPI, typename OutT, int FA, int FB, int F>
+__device__ __forceinline__ void fp8_w4_body(const Fp8GemmArgs& p, DLLM_LDS char* lds) {
+  constexpr int TS = 32 * F, OPB = TS * 128, STAGE = 2 * OPB, STAGES = 4;
+  constexpr bool EXACT = sizeof(OutT) == 4;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
+  const int tiles_m = (p.M + TS - 1) / TS, tiles_n = (p.N + TS - 1) / TS;
+  const int bid = xcd_remap(blockIdx.x, gridDim.x);
+  const int width = 4 * tiles_n, first = bid / width * 4, gsz = min(tiles_m - first, 4);
+  const int m0 = (first + bid % width % gsz) * TS, n0 = (bid % width / gsz) * TS;
+  const int k0 = (int)((long)p.nk * blockIdx.y / p.ksplit), nk = (int)((long)p.nk * (blockIdx.y + 1) / p.ksplit) - k0;
+
+  uint32_t ao[F], bo[F];
+#pragma unroll
+  for (int i = 0; i < F; ++i) {
+    const int s = 8 * (wid + 4 * i) + (lane >> 3);
+    const int w = s / (16 * F), in = s - w * 16 * F;
+    const int row = w * 16 * F + F * (in & 15) + (in >> 4), c = (lane & 7) ^ ((s >> 1) & 7);
+    ao[i] = (uint32_t)((long)min(row, p.M - 1 - m0) * p.lda + c * 16);
+    bo[i] = (uint32_t)((long)min(row, p.N - 1 - n0) * p.ldb + c * 16);
+  }
+  const char* A = (const char*)p.A + (long)m0 * p.lda + (long)k0 * 128;
+  const char* B = (const char*)p.B + (long)n0 * p.ldb + (long)k0 * 128;
+  auto fetch = [&](int i, int kt, int slot) {       // piece i of the step (0 .. 2F - 1: A's, then B's); past the end: the last
+    const long ko = (long)min(kt, nk - 1) * 128;
+    DLLM_LDS char* d = lds + slot * STAGE;
+    if (i < F) n8_dma(A + ko, ao[i], d + (wid + 4 * i) * 1024);
+    else n8_dma(B + ko, bo[i - F], d + OPB + (wid + 4 * (i - F)) * 1024);
+  };
+  // scales: the lane's F rows of A and of B; a word that would pass the end of its row starts earlier and is shifted
+  const int ra = m0 + wr * 16 * F + F * i15, rb = n0 + wc * 16 * F + F * i15;
+  const int oa = max(0, min(ra, p.M - F)), ob = max(0, min(rb, p.N - F));
+  const int sha = min(8 * (ra - oa), 8 * F - 8), shb = min(8 * (rb - ob), 8 * F - 8);
+  auto scales = [&](const uint8_t* s, long ld, int kt, int off) {
+    const uint8_t* q = s + (long)(k0 + min(kt, nk - 1)) * ld + off;
+    if constexpr (F == 4) return (uint32_t)*(const u32_any*)q;
+    else return (uint32_t)*(const u16_any*)q;
+  };
+  const uint32_t lb = (uint32_t)(uintptr_t)lds;
+  const int sw = (i15 >> 1) & 7;
+  const uint32_t la[2] = {lb + (wr * 16 * F + i15) * 128 + ((g ^ sw) << 4), lb + (wr * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
+  const uint32_t lbb[2] = {lb + OPB + (wc * 16 * F + i15) * 128 + ((g ^ sw) << 4),
+                           lb + OPB + (wc * 16 * F + i15) * 128 + (((4 + g) ^ sw) << 4)};
+  N8Frag xa[2][F], xb[2][F];
+  uint32_t wa[2], wb[2];
+  f32x4_t acc[F][F];
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int k = 0; k < F; ++k) acc[i][k] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto read = [&](auto par, auto j, uint32_t off) {   // read j of a step's 4F
+    constexpr int f = j.value >> 1, h = j.value & 1;
+    if constexpr (f < F) n8_read<f * 2048>(h ? xa[par.value][f].hi : xa[par.value][f].lo, la[h] + off);
+    else n8_read<(f - F) * 2048>(h ? xb[par.value][f - F].hi : xb[par.value][f - F].lo, lbb[h] + off);
+  };
+  auto upto = [](auto n, auto f) {
+    [&]<int... J>(std::integer_sequence<int, J...>) { (f(std::integral_constant<int, J>{}), ...); }(std::make_integer_sequence<int, decltype(n)::value>{});
+  };
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, 1>;
+  using NR = std::integral_constant<int, 4 * F>;
+  using NQ = std::integral_constant<int, F * F>;
+  if (nk > 0) {
+    wa[0] = scales(p.SA, p.ldsa, 0, oa);
+    wb[0] = scales(p.SB, p.ldsb, 0, ob);
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s)
+#pragma unroll
+      for (int i = 0; i < 2 * F; ++i) fetch(i, s, s);
+    if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    N8_BARRIER();
+    upto(NR{}, [&](auto j) { read(I0{}, j, 0u); });
+    N8_LDS_WAIT();
+    int slot = 0;
+    // step kt: its fragments are in registers and its LDS slot is free; read step kt + 1, fetch step kt + 4
+    auto one = [&](auto par, auto other, int kt) {
+      if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+      N8_BARRIER();
+      const int fs = slot;
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+      const uint32_t off = (uint32_t)(slot * STAGE);
+      wa[other.value] = scales(p.SA, p.ldsa, kt + 1, oa);
+      wb[other.value] = scales(p.SB, p.ldsb, kt + 1, ob);
+      upto(NR{}, [&](auto j) { read(other, j, off); });
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2 * F; ++i) fetch(i, kt + STAGES, fs);
+      __builtin_amdgcn_sched_barrier(0);
+      const uint32_t a = wa[par.value] >> sha, b = wb[par.value] >> shb;
+      if constexpr (!EXACT) {
+        upto(NQ{}, [&](auto q) {
+          constexpr int i = q.value / F, k = q.value % F;
+          const N8Frag &fa = xa[par.value][i], &fb = xb[par.value][k];
+          const i32x8_t x = __builtin_shufflevector(fa.lo, fa.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          const i32x8_t y = __builtin_shufflevector(fb.lo, fb.hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[i][k] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(y, x, acc[i][k], FB, FA, k, (int)b, i, (int)a);
+        });
+      } else {
+        auto scale = [](uint32_t w, int i) { return __uint_as_float((w >> (8 * i) & 255u) << 23); };
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          auto pick = [&](const N8Frag& f, int k) { return s < 2 ? f.lo[2 * (s & 1) + k] : f.hi[2 * (s & 1) + k]; };
+          bf16x8_t y[F];
+#pragma unroll
+          for (int k = 0; k < F; ++k) y[k] = codes8<FB>(pick(xb[par.value][k], 0), pick(xb[par.value][k], 1), scale(b, k));
+#pragma unroll
+          for (int i = 0; i < F; ++i) {
+            const bf16x8_t x = codes8<FA>(pick(xa[par.value][i], 0), pick(xa[par.value][i], 1), scale(a, i));
+#pragma unroll
+            for (int k = 0; k < F; ++k) acc[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[k], x, acc[i][k], 0, 0, 0);
+          }
+        }
+      }
+      N8_LDS_WAIT();
+    };
+    for (int kt = 0; kt < nk; kt += 2) {
+      one(I0{}, I1{}, kt);
+      if (kt + 1 < nk) one(I1{}, I0{}, kt + 1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+
+  // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
+  const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
+  const bool fast = f8_aligned<OutT>(p) && n0 + TS <= p.N && m0 + TS <= p.M;
+#pragma unroll
+  for (int i = 0; i < F; ++i)
+#pragma unroll
+    for (int c8 = 0; c8 < F / 2; ++c8) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = acc[i][(8 * c8 + e) % F][(8 * c8 + e) / F];
+      if (p.ksplit > 1) {
+        const int m = mb + i, n = nb + 8 * c8;
+        if (m < p.M) {
+          float* o = p.ws + (long)blockIdx.y * p.M * p.N + (long)m * p.N + n;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < p.N) o[e] = v[e];
+        }
+      } else {
+        f8_epi8<EPI, OutT>(p, fast, mb + i, nb + 8 * c8, v);
+      }
+    }
+}
+
+constexpr int fp8_w4_lds(int f) { return 4 * 2 * 32 * f * 128; }
+extern __shared__ __attribute__((aligned(16))) char fp8_dyn_lds[];
+// Dynamic LDS (128 KiB, one block per CU) and a bound of two blocks: the compiler then stays within 256 registers.  Left with
+// 512 it keeps the accumulators in the accumulation file and copies each one around its matrix instruction.
+template <int EPI, typename OutT, int FA, int FB>
+__global__ __launch_bounds__(256, 2) void fp8_gemm_128(Fp8GemmArgs p) {
+  fp8_w4_body<EPI, OutT, FA, FB, 4>(p, (DLLM_LDS char*)fp8_dyn_lds);
+}
+template <int EPI, typename OutT, int FA, int FB>
+__global__ __launch_bounds__(256, 2) void fp8_gemm_64(Fp8GemmArgs p) {
+  __shared__ __attribute__((aligned(16))) char smem[fp8_w4_lds(2)];
+  fp8_w4_body<EPI, OutT, FA, FB, 2>(p, (DLLM_LDS char*)smem);
+}
+
+// the K slices' sums, in the order of K, and the epilogue; a thread per element
 template <int EPI, typename OutT>
-static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s) {
-  const long tiles = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)tiles), block(256);
-  {
-    const long big = (long)((p.M + 255) / 256) * ((p.N + 255) / 256);
-    if (p.nk > 0 && p.M >= 4 && p.N >= 2 && big >= 128) {
-      const dim3 g2((unsigned)big), b2(512);
-      if (fa == F8_E4M3 && fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E4M3, F8_E4M3>), g2, b2, 0, s, p);
-      else if (fa == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E4M3, F8_E5M2>), g2, b2, 0, s, p);
-      else if (fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E5M2, F8_E4M3>), g2, b2, 0, s, p);
-      else hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, F8_E5M2, F8_E5M2>), g2, b2, 0, s, p);
-      return hipGetLastError();
+__global__ __launch_bounds__(256) void fp8_join(Fp8GemmArgs p) {
+  const long n = (long)p.M * p.N;
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+    float s = p.ws[i];
+    for (int k = 1; k < p.ksplit; ++k) s += p.ws[(long)k * n + i];
+    f8_epi1<EPI, OutT>(p, (int)(i / p.N), (int)(i % p.N), s);
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// few rows of A (SWAP: of B), at most 16 MT: 16 rows of the other operand per block, the K steps dealt to its 8 waves
+//
+// Bound by reading the long operand once (and by latency: everything a wave needs for 4 steps is requested at once).
+// Fragments go from memory to registers (a step's line of a row is read by the 4 lanes of its row), the waves' sums are
+// added in LDS in the order of the waves.
+// ----------------------------------------------------------------------------------------------
+template <int EPI, typename OutT, int FA, int FB, int MT, bool SWAP>
+__global__ __launch_bounds__(512) void fp8_gemm_rows(Fp8GemmArgs p) {
+  __shared__ f32x4_t part[8][MT][64];
+  constexpr bool EXACT = sizeof(OutT) == 4;
+  constexpr int FS = SWAP ? FB : FA, FL = SWAP ? FA : FB;        // formats of the short and the long operand
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, i15 = lane & 15, g = lane >> 4;
+  const uint8_t *L = SWAP ? p.A : p.B, *SL = SWAP ? p.SA : p.SB, *S = SWAP ? p.B : p.A, *SS = SWAP ? p.SB : p.SA;
+  const long ldl = SWAP ? p.lda : p.ldb, ldsl = SWAP ? p.ldsa : p.ldsb, lds = SWAP ? p.ldb : p.lda, ldss = SWAP ? p.ldsb : p.ldsa;
+  const int nl = SWAP ? p.M : p.N, ns = SWAP ? p.N : p.M;
+  const int l0 = blockIdx.x * 16, rl = min(l0 + i15, nl - 1);
+  const uint8_t* lp = L + (long)rl * ldl + g * 16;
+  int rs[MT];
+  const uint8_t* sp[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    rs[i] = min(16 * i + i15, ns - 1);
+    sp[i] = S + (long)rs[i] * lds + g * 16;
+  }
+  f32x4_t acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto load = [](const uint8_t* q) {
+    const n8_i32x4 lo = *(const n8_i32x4*)q, hi = *(const n8_i32x4*)(q + 64);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  constexpr int U = MT == 4 ? 2 : 4;
+#pragma unroll U
+  for (int kt = w; kt < p.nk; kt += 8) {
+    const i32x8_t fl = load(lp + (long)kt * 128);
+    const int sl = SL[(long)kt * ldsl + rl];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const i32x8_t fs = load(sp[i] + (long)kt * 128);
+      const int ss = SS[(long)kt * ldss + rs[i]];
+      if constexpr (!EXACT) {
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fl, fs, acc[i], FL, FS, 0, sl, 0, ss);
+      } else {
+        const float a = __uint_as_float((uint32_t)ss << 23), b = __uint_as_float((uint32_t)sl << 23);
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<FL>(fl[2 * s], fl[2 * s + 1], b),
+                                                           codes8<FS>(fs[2 * s], fs[2 * s + 1], a), acc[i], 0, 0, 0);
+      }
     }
   }
-  if (fa == F8_E4M3 && fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E4M3, F8_E4M3>), grid, block, 0, s, p);
-  else if (fa == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E4M3, F8_E5M2>), grid, block, 0, s, p);
-  else if (fb == F8_E4M3) hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E5M2, F8_E4M3>), grid, block, 0, s, p);
-  else hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, F8_E5M2, F8_E5M2>), grid, block, 0, s, p);
+#pragma unroll
+  for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[i];
+  __syncthreads();
+  if (w < MT) {
+    f32x4_t v = part[0][w][lane];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) v += part[k][w][lane];
+    const int s = 16 * w + i15, l = l0 + 4 * g;               // lane: rows l .. l + 3 of the long operand, row s of the short
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = SWAP ? l + r : s, n = SWAP ? s : l + r;
+      if (m < p.M && n < p.N) f8_epi1<EPI, OutT>(p, m, n, v[r]);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------
+// choice and launch
+// ----------------------------------------------------------------------------------------------
+static int fp8_cus() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
+    return v;
+  }();
+  return n;
+}
+
+template <int EPI, typename OutT, int FA, int FB>
+static hipError_t launch_fp8_f(Fp8GemmArgs p, hipStream_t s) {
+  const int few = min(p.M, p.N);
+  if (few <= 64) {
+    const bool swap = p.N < p.M;
+    const dim3 grid((unsigned)((max(p.M, p.N) + 15) / 16)), block(512);
+    auto go = [&](auto mt, auto sw) {
+      hipLaunchKernelGGL((fp8_gemm_rows<EPI, OutT, FA, FB, decltype(mt)::value, decltype(sw)::value>), grid, block, 0, s, p);
+    };
+    using T = std::true_type;
+    using N = std::false_type;
+    auto by = [&](auto sw) {
+      if (few <= 16) go(std::integral_constant<int, 1>{}, sw);
+      else if (few <= 32) go(std::integral_constant<int, 2>{}, sw);
+      else go(std::integral_constant<int, 4>{}, sw);
+    };
+    if (swap) by(T{});
+    else by(N{});
+    return hipGetLastError();
+  }
+  const int ts = p.tile;
+  const long tiles = (long)((p.M + ts - 1) / ts) * ((p.N + ts - 1) / ts);
+  if (tiles > 0x7fffffffL) return hipErrorInvalidValue;
+  if (ts == 256) hipLaunchKernelGGL((fp8_gemm_256<EPI, OutT, FA, FB>), dim3((unsigned)tiles), dim3(512), 0, s, p);
+  else if (ts == 128) {
+    const hipError_t e = lds_opt_in((const void*)fp8_gemm_128<EPI, OutT, FA, FB>, fp8_w4_lds(4));
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((fp8_gemm_128<EPI, OutT, FA, FB>), dim3((unsigned)tiles, p.ksplit), dim3(256), fp8_w4_lds(4), s, p);
+  }
+  else hipLaunchKernelGGL((fp8_gemm_64<EPI, OutT, FA, FB>), dim3((unsigned)tiles, p.ksplit), dim3(256), 0, s, p);
+  if (p.ksplit > 1) {
+    const long n = (long)p.M * p.N;
+    hipLaunchKernelGGL((fp8_join<EPI, OutT>), dim3((unsigned)min((n + 255) / 256, 2048L)), dim3(256), 0, s, p);
+  }
   return hipGetLastError();
+}
+
+template <int EPI, typename OutT>
+static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s) {
+  if (fa == F8_E4M3) return fb == F8_E4M3 ? launch_fp8_f<EPI, OutT, F8_E4M3, F8_E4M3>(p, s) : launch_fp8_f<EPI, OutT, F8_E4M3, F8_E5M2>(p, s);
+  return fb == F8_E4M3 ? launch_fp8_f<EPI, OutT, F8_E5M2, F8_E4M3>(p, s) : launch_fp8_f<EPI, OutT, F8_E5M2, F8_E5M2>(p, s);
+}
+
+// Tile and number of K slices: the least time for whole rounds of CUs, in microseconds measured on full rounds: a K step of
+// 128 on one CU (bf16 results / fp32 results), a round's beginning and end, and the slices' partial sums at 1.5 TB/s.
+static void fp8_plan(int M, int N, int nk, bool exact, int& tile, int& ksplit) {
+  struct { int ts, blocks; float fast, exact; } kinds[] = {{256, 1, 1.45f, 3.0f}, {128, 1, 0.42f, 0.75f}, {64, 2, 0.30f, 0.40f}};
+  float best = 1e30f;
+  tile = 128;
+  ksplit = 1;
+  const long cus = fp8_cus();
+  for (auto& k : kinds) {
+    const long tiles = (long)((M + k.ts - 1) / k.ts) * ((N + k.ts - 1) / k.ts);
+    for (int s = 1; s <= 8; s *= 2) {
+      if (s > 1 && (k.ts == 256 || nk < 4 * s)) break;
+      const float rounds = (float)((tiles * s + cus * k.blocks - 1) / (cus * k.blocks));
+      float t = rounds * ((float)((nk + s - 1) / s) * (exact ? k.exact : k.fast) + 5.f);
+      if (s > 1) t += 5.f + (float)M * (float)N * (float)(8 * s) / 1.5e6f;
+      if (t < best) { best = t; tile = k.ts; ksplit = s; }
+    }
+  }
 }
 
 }  // namespace dllm
@@ -683,10 +870,19 @@ int dllm_fp8_dequantize(const void* q, long ldq, const void* sq, long ldsq, int 
   return (int)hipGetLastError();
 }
 
+// tile size (low 16 bits) and K slices (high 16) that dllm_fp8_gemm should be given; ksplit > 1 needs ksplit * M * N floats
+int dllm_fp8_gemm_plan(int M, int N, int nk, int out_dtype) {
+  int tile, ksplit;
+  fp8_plan(M, N, nk, out_dtype == DT_F32, tile, ksplit);
+  if (nk == 0 && tile == 256) tile = 128;
+  return tile | ksplit << 16;
+}
+
 // C [M, N] (out_dtype) from A [M, 128 nk], B [N, 128 nk].  epi: EPI_STORE / EPI_ACT / EPI_DACT.
 int dllm_fp8_gemm(const void* A, long lda, const void* SA, long ldsa, int fa, const void* B, long ldb, const void* SB,
                   long ldsb, int fb, void* C, long ldc, int out_dtype, const void* aux, void* aux_out, long ldaux, int M,
-                  int N, int nk, float alpha, float beta, int epi, int act, void* stream) {
+                  int N, int nk, float alpha, float beta, int epi, int act, int tile, int ksplit, float* ws,
+                  void* stream) {
   if (M <= 0 || N <= 0 || nk < 0 || nk > (1 << 24) || (out_dtype != DT_BF16 && out_dtype != DT_F32)) return -1;
   if (fa < 0 || fa > 1 || fb < 0 || fb > 1 || ldc < N) return -1;
   if (nk > 0 && ((uintptr_t)A % 16 || (uintptr_t)B % 16 || lda % 16 || ldb % 16 || lda < 128L * nk || ldb < 128L * nk ||
@@ -697,7 +893,13 @@ int dllm_fp8_gemm(const void* A, long lda, const void* SA, long ldsa, int fa, co
   if (epi == EPI_DACT && aux == nullptr) return -1;
   if ((aux || aux_out) && ldaux < N) return -1;
   Fp8GemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)SA, ldsa, (const uint8_t*)B, ldb, (const uint8_t*)SB, ldsb,
-                C, ldc, aux, aux_out, ldaux, M, N, nk, alpha, beta, act};
+                C, ldc, aux, aux_out, ldaux, M, N, nk, alpha, beta, act, tile, ksplit, ws};
+  if (min(M, N) > 64) {
+    // the buffer-form fetches reach 2^31 bytes from a tile's first row; scale words span 4 (2) rows, which these have
+    if ((tile != 64 && tile != 128 && tile != 256) || ksplit < 1 || ksplit > 8 || (ksplit > 1 && (ws == nullptr || tile == 256)))
+      return -1;
+    if (max(lda, ldb) > (0x7fffffffL - 4096) / 256 || (nk == 0 && tile == 256)) return -1;
+  }
   hipStream_t s = (hipStream_t)stream;
   const bool bf = out_dtype == DT_BF16;
   switch (epi) {

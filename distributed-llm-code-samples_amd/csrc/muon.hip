@@ -468,10 +468,8 @@ template <int F> struct W4 {
 };
 
 template <int EPI, int F>
-__global__ __launch_bounds__(256, 1) void ns_gemm_w4(NsGemm p) {
+__device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) {
   using W = W4<F>;
-  __shared__ __attribute__((aligned(16))) char smem[W::STAGES * W::STAGE];
-  DLLM_LDS char* lds = (DLLM_LDS char*)smem;
   const int t = threadIdx.x, lane = t & 63;
   const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
   const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
@@ -638,6 +636,18 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_w4(NsGemm p) {
   }
 }
 
+// 128 x 128: dynamic LDS (128 KiB, one block per CU) and a bound of two blocks, so that the compiler stays within 256
+// registers; left with 512 it keeps these 64 accumulators in the accumulation file and copies each one around its matrix
+// instruction.  192 x 192 tiles (144 accumulators) need both files and get no copies.
+extern __shared__ __attribute__((aligned(16))) char ns_dyn_lds[];
+template <int EPI>
+__global__ __launch_bounds__(256, 2) void ns_gemm_128(NsGemm p) { ns_w4_body<EPI, 4>(p, (DLLM_LDS char*)ns_dyn_lds); }
+template <int EPI>
+__global__ __launch_bounds__(256, 1) void ns_gemm_192(NsGemm p) {
+  __shared__ __attribute__((aligned(16))) char smem[W4<6>::STAGES * W4<6>::STAGE];
+  ns_w4_body<EPI, 6>(p, (DLLM_LDS char*)smem);
+}
+
 static int ns_cus() {
   static const int n = [] {
     int dev = 0, v = 0;
@@ -660,8 +670,13 @@ static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
   const long grid = (long)B * ns_tiles(p, ts);
   if (grid > 0x7fffffffL) return hipErrorInvalidValue;
   if (ts == 256) hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3((unsigned)grid), dim3(512), 0, s, p);
-  else if (ts == 192) hipLaunchKernelGGL((ns_gemm_w4<EPI, 6>), dim3((unsigned)grid), dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((ns_gemm_w4<EPI, 4>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else if (ts == 192) hipLaunchKernelGGL((ns_gemm_192<EPI>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  else {
+    constexpr int lds = W4<4>::STAGES * W4<4>::STAGE;
+    const hipError_t e = lds_opt_in((const void*)ns_gemm_128<EPI>, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((ns_gemm_128<EPI>), dim3((unsigned)grid), dim3(256), lds, s, p);
+  }
   return hipGetLastError();
 }
 

@@ -59,6 +59,11 @@ __device__ __forceinline__ void n8_dma(const char* src, uint32_t off, DLLM_LDS c
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DLLM_LDS void*)dst, 16, (int)off, 0, 0, 0);
 }
 
+// dynamic LDS beyond 64 KiB is allowed per kernel, once
+static inline hipError_t lds_opt_in(const void* kernel, int bytes) {
+  return hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 struct N8Frag { n8_i32x4 lo, hi; };        // 32 bytes of a row: 16-B chunks g and 4 + g of the K step
 
 // byte offsets (within the operand, from the tile's first row) of the two LDS-DMA pieces a wave fetches of a half-tile.

@@ -95,7 +95,8 @@ def product_check(got, qa, qb, alpha=1.0, beta=0.0, c=None, ref=None, mag_gain=1
 
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 128), (3, 5, 129), (16, 1000, 640), (64, 64, 256), (127, 129, 255),
                                    (128, 128, 384), (200, 333, 1537), (256, 256, 256), (300, 512, 2048), (512, 768, 1024),
-                                   (1, 4096, 512), (33, 2000, 300), (1030, 260, 140)])
+                                   (1, 4096, 512), (33, 2000, 300), (1030, 260, 140), (65, 65, 100), (1000, 16, 700),
+                                   (1000, 40, 1300), (17, 1000, 8200), (200, 70, 16500), (100, 100, 5000), (66, 513, 2500)])
 @pytest.mark.parametrize("fa,fb", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
 def test_gemm(M, N, K, fa, fb, out):
@@ -153,6 +154,31 @@ def test_gemm_into_a_view_and_odd_strides():
             buf = torch.full((132, ldc), 5.0, dtype=dt, device=DEV)
             product_check(fp8.gemm_fp8(pa, pb, buf[1:131, :147]), pa, pb)
             assert (buf[0] == 5).all() and (buf[131] == 5).all() and (buf[:, 147:] == 5).all()
+
+
+def test_gemm_every_tile_and_slice(monkeypatch):
+    """The plan's choices one by one on sizes that it would not choose them for."""
+    for M, N, K in ((65, 70, 130), (300, 290, 1290), (257, 129, 2100)):
+        qa, qb = fp8.quantize_fp8(rand(M, K, 1).to(DEV), "e5m2"), fp8.quantize_fp8(rand(N, K, 2).to(DEV))
+        for tile, ksplit in ((64, 1), (128, 1), (256, 1), (64, 2), (128, 4), (64, 8), (128, 1)):
+            if ksplit > 1 and K < 128 * ksplit:
+                continue
+            monkeypatch.setattr(fp8, "_plan", lambda *_: (tile, ksplit))
+            for out in (torch.bfloat16, torch.float32):
+                h = torch.empty(M, N, dtype=out, device=DEV)
+                product_check(fp8.gemm_fp8(qa, qb, out_dtype=out), qa, qb)
+                a = fp8.gemm_fp8(qa, qb, out_dtype=out, epi="act", act="relu", aux_out=h)
+                product_check(h, qa, qb)
+                assert torch.equal(a, h.clamp(min=0))
+
+
+def test_gemm_no_depth():
+    q, w = fp8.quantize_fp8(torch.empty(70, 0, device=DEV)), fp8.quantize_fp8(torch.empty(80, 0, device=DEV))
+    assert torch.equal(fp8.gemm_fp8(q, w), torch.zeros(70, 80, dtype=torch.bfloat16, device=DEV))
+    c = torch.ones(70, 80, device=DEV)
+    assert torch.equal(fp8.gemm_fp8(q, w, c, beta=0.5), torch.full((70, 80), 0.5, device=DEV))
+    one = fp8.quantize_fp8(torch.empty(1, 0, device=DEV))
+    assert torch.equal(fp8.gemm_fp8(one, w), torch.zeros(1, 80, dtype=torch.bfloat16, device=DEV))
 
 
 def test_single_row_with_arbitrary_strides():
