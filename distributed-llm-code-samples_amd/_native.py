@@ -66,7 +66,7 @@ _SIGS = {
     "dllm_orthogonalize": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_long,
                                    c_void_p]),
     "dllm_muon_step": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_float,
-                               c_float, c_int, c_float, c_float, c_float, c_void_p, c_long, c_void_p]),
+                               c_float, c_int, c_float, c_float, c_float, c_int, c_void_p, c_long, c_void_p]),
     "dllm_abi_version": (c_int, []),
 }
 _OPTIONAL_SIGS: dict = {}

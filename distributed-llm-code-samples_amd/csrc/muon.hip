@@ -50,7 +50,12 @@ struct MuonIn {
   float beta, gscale;
   int nesterov;
   int R, C;
+  int il, B;                  // il > 0: the rows of the B matrices alternate in blocks of il (one [B R][C] tensor)
 };
+// first element of row r of matrix z
+__device__ __forceinline__ long muon_row(int il, int B, int R, int C, int z, int r) {
+  return (il ? ((long)(r / il) * B + z) * il + r % il : (long)z * R + r) * C;
+}
 
 __device__ __forceinline__ float ld_g(const MuonIn& p, long i) {
   return p.gdt == DT_BF16 ? bf2f(((const uint16_t*)p.g)[i]) : ((const float*)p.g)[i];
@@ -90,12 +95,14 @@ __device__ __forceinline__ f32x4_t muon_u4(const MuonIn& p, long i) {
 // momentum update and the partial sums of u^2 (64-bit: gradients of any magnitude, and a sum that does not depend on how it
 // is cut).  grid (NS_PARTS, B).  Bound by HBM: one read of g (and of the momentum, and its write)
 template <int KIND, bool VEC>
-__device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, long base, long n) {
+__device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, int z, long n) {
   double s = 0.0;
+  const long chunk = (long)p.il * p.C;                       // contiguous elements of one matrix
+  auto at = [&](long i) { return p.il ? (i / chunk * p.B + z) * chunk + i % chunk : (long)z * n + i; };
   const long n4 = VEC ? n >> 2 : 0, stride = (long)gridDim.x * blockDim.x, t0 = (long)blockIdx.x * blockDim.x + threadIdx.x;
 #pragma unroll 4
   for (long j = t0; j < n4; j += stride) {
-    const long i = base + 4 * j;
+    const long i = at(4 * j);
     if constexpr (KIND == NS_MUON) {
       const f32x4_t g = ld_g4<VEC>(p, i);
       f32x4_t m = *(const f32x4_t*)(p.mom + i);
@@ -112,7 +119,8 @@ __device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, long base, lo
       for (int k = 0; k < 4; ++k) s += (double)u[k] * (double)u[k];
     }
   }
-  for (long i = base + 4 * n4 + t0; i < base + n; i += stride) {
+  for (long j = 4 * n4 + t0; j < n; j += stride) {
+    const long i = at(j);
     if constexpr (KIND == NS_MUON) p.mom[i] = fmaf(p.beta, p.mom[i], p.gscale * ld_g(p, i));
     const double u = (double)muon_u<KIND>(p, i);
     s += u * u;
@@ -129,8 +137,11 @@ __device__ __forceinline__ bool muon_vec(const MuonIn& p, long base) {
 template <int KIND>
 __global__ __launch_bounds__(1024) void muon_sumsq_kernel(MuonIn p, double* part) {
   __shared__ double red[16];
-  const long n = (long)p.R * p.C, base = (long)blockIdx.y * n;
-  double s = muon_vec<KIND>(p, base) ? muon_sumsq_part<KIND, true>(p, base, n) : muon_sumsq_part<KIND, false>(p, base, n);
+  const int z = blockIdx.y;
+  const long n = (long)p.R * p.C, base = muon_row(p.il, p.B, p.R, p.C, z, 0);
+  // (alternating rows: whole vectors in every block of rows)
+  const bool vec = muon_vec<KIND>(p, base) && (p.il == 0 || p.il * (long)p.C % 8 == 0);
+  double s = vec ? muon_sumsq_part<KIND, true>(p, z, n) : muon_sumsq_part<KIND, false>(p, z, n);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -162,13 +173,13 @@ __global__ __launch_bounds__(256) void ns_split_kernel(MuonIn p, const double* p
   f16* so = same + (long)blockIdx.z * 2 * plane;
   f16* to = tr + (long)blockIdx.z * 2 * plane;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, q = t >> 4, j = 4 * (t & 15);
-  const bool vec = p.C % 8 == 0 && muon_vec<KIND>(p, (long)blockIdx.z * p.R * p.C);
+  const bool vec = p.C % 8 == 0 && muon_vec<KIND>(p, 0);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + 16 * i + q, c = c0 + j;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     if (r < p.R && c < p.C) {
-      const long o = ((long)blockIdx.z * p.R + r) * p.C + c;
+      const long o = muon_row(p.il, p.B, p.R, p.C, blockIdx.z, r) + c;
       if (vec) {
         v = muon_u4<KIND, true>(p, o);
       } else {
@@ -220,6 +231,7 @@ struct NsGemm {
   f16* outT; long ldt, pt, bt;         // transposed planes (NS_PLANES_T)
   const f16* aux; float cb, ca;        // NS_POLY: A's planes (out's layout), b's factor, a on the diagonal
   void* C; int cdt, R, Cc, vec;        // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
+  int il, nb;                          // NS_STEP: alternating rows, as in MuonIn
   float* w; uint16_t* copy; int16_t* lo; float decay, rate;   // NS_STEP: fp32 master (+ bf16 copy), or split (lo, copy)
   int sym;                             // the product is symmetric: tiles on and below the diagonal, mirrored on writing
 };
@@ -228,7 +240,7 @@ struct NsGemm {
 template <int EPI>
 __device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n, const float (&v)[8]) {
   if (m >= p.R || n >= p.Cc) return;
-  const long o = ((long)z * p.R + m) * p.Cc + n;
+  const long o = muon_row(p.il, p.nb, p.R, p.Cc, z, m) + n;
   if (p.vec) {   // whole rows of 8, 16-byte aligned
     if constexpr (EPI == NS_OUT) {
       if (p.cdt == DT_BF16) {
@@ -453,7 +465,7 @@ __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
 }
 
 // ----------------------------------------------------------------------------------------------
-// 128x128 (F = 4) and 192x192 (F = 6) tiles: four waves, one per SIMD, each 16F x 16F
+// 64x64 (F = 2), 128x128 (F = 4) and 192x192 (F = 6) tiles: four waves, one per SIMD, each 16F x 16F
 //
 // For products whose 256x256 tiles do not fill the CUs: a symmetric 4096 x 4096 product has 136 of those and takes one
 // round on 256 CUs as the full 256 tiles do, but 253 of 192 x 192, one round of 0.56 of the work.
@@ -464,7 +476,8 @@ __global__ __launch_bounds__(512, 2) void ns_gemm_256(NsGemm p) {
 // ----------------------------------------------------------------------------------------------
 template <int F> struct W4 {
   static constexpr int TS = 32 * F, OPB = TS * 128, STAGE = 2 * OPB;      // bytes of an operand's / a step's LDS
-  static constexpr int STAGES = F == 4 ? 4 : 3, PIECES = F;               // 1-KiB LDS-DMA pieces per wave and operand
+  static constexpr int STAGES = F == 6 ? 3 : 4;
+  static constexpr int LDS = STAGES * STAGE;
 };
 
 template <int EPI, int F>
@@ -542,11 +555,14 @@ __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) 
     for (int i = 0; i < F; ++i) fetch_b(i, s);
     next();
   }
-  auto landed = [] {   // all but the youngest STAGES - 2 (2F fetches each) steps in flight have landed
-    if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+  auto landed = [] {   // all but the youngest STAGES - 2 steps (2F fetches each) in flight have landed
+    if constexpr (F == 2) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if constexpr (F == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
   };
-  asm volatile("s_waitcnt vmcnt(24)" ::: "memory");   // (STAGES - 1) * 2F: step 0 has landed
+  // (STAGES - 1) * 2F: step 0 has landed
+  if constexpr (F == 2) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
   N8_BARRIER();
   upto(NR{}, [&](auto j) { read(I0{}, j, 0u); });
   N8_LDS_WAIT();
@@ -558,7 +574,7 @@ __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) 
     const int fs = slot;
     slot = slot + 1 == W::STAGES ? 0 : slot + 1;
     const uint32_t off = (uint32_t)(slot * W::STAGE);
-    constexpr int PR = F == 4 ? 1 : 2;             // matrix instructions per read, then two per fetch
+    constexpr int PR = F / 2 - (F < 6);            // matrix instructions per read (0, 1, 2), then two per fetch
     upto(NR{}, [&](auto j) {
       read(other, j, off);
       __builtin_amdgcn_sched_barrier(0);
@@ -643,8 +659,13 @@ extern __shared__ __attribute__((aligned(16))) char ns_dyn_lds[];
 template <int EPI>
 __global__ __launch_bounds__(256, 2) void ns_gemm_128(NsGemm p) { ns_w4_body<EPI, 4>(p, (DLLM_LDS char*)ns_dyn_lds); }
 template <int EPI>
+__global__ __launch_bounds__(256, 2) void ns_gemm_64(NsGemm p) {
+  __shared__ __attribute__((aligned(16))) char smem[W4<2>::LDS];
+  ns_w4_body<EPI, 2>(p, (DLLM_LDS char*)smem);
+}
+template <int EPI>
 __global__ __launch_bounds__(256, 1) void ns_gemm_192(NsGemm p) {
-  __shared__ __attribute__((aligned(16))) char smem[W4<6>::STAGES * W4<6>::STAGE];
+  __shared__ __attribute__((aligned(16))) char smem[W4<6>::LDS];
   ns_w4_body<EPI, 6>(p, (DLLM_LDS char*)smem);
 }
 
@@ -663,19 +684,24 @@ static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
   // rounds: 128 x 128 is bound by LDS, the larger ones by the matrix units' power), and of a round's beginning and end
   const long cus = ns_cus();
   const float steps = 3.f * (float)(p.K >> 6);
-  auto time = [&](int ts, float step) { return (float)(((long)B * ns_tiles(p, ts) + cus - 1) / cus) * (steps * step + 6.f); };
-  const float t128 = time(128, 0.40f), t192 = time(192, 0.75f);
-  const float t256 = p.M % 256 == 0 && p.N % 256 == 0 ? time(256, 1.5f) : 1e30f;
-  const int ts = t256 <= t128 && t256 <= t192 ? 256 : t192 < t128 ? 192 : 128;
-  const long grid = (long)B * ns_tiles(p, ts);
+  auto time = [&](int ts, long per_cu, float step) {
+    return (float)(((long)B * ns_tiles(p, ts) + cus * per_cu - 1) / (cus * per_cu)) * (steps * step + 5.f);
+  };
+  const bool whole = p.M % 256 == 0 && p.N % 256 == 0;
+  const float t[4] = {time(64, 2, 0.24f), time(128, 1, 0.40f), time(192, 1, 0.85f), whole ? time(256, 1, 1.5f) : 1e30f};
+  int best = 0;
+  for (int i = 1; i < 4; ++i)
+    if (t[i] < t[best]) best = i;
+  const long grid = (long)B * ns_tiles(p, 64 * (best + 1));
   if (grid > 0x7fffffffL) return hipErrorInvalidValue;
-  if (ts == 256) hipLaunchKernelGGL((ns_gemm_256<EPI>), dim3((unsigned)grid), dim3(512), 0, s, p);
-  else if (ts == 192) hipLaunchKernelGGL((ns_gemm_192<EPI>), dim3((unsigned)grid), dim3(256), 0, s, p);
+  const dim3 g((unsigned)grid);
+  if (best == 3) hipLaunchKernelGGL((ns_gemm_256<EPI>), g, dim3(512), 0, s, p);
+  else if (best == 2) hipLaunchKernelGGL((ns_gemm_192<EPI>), g, dim3(256), 0, s, p);
+  else if (best == 0) hipLaunchKernelGGL((ns_gemm_64<EPI>), g, dim3(256), 0, s, p);
   else {
-    constexpr int lds = W4<4>::STAGES * W4<4>::STAGE;
-    const hipError_t e = lds_opt_in((const void*)ns_gemm_128<EPI>, lds);
+    const hipError_t e = lds_opt_in((const void*)ns_gemm_128<EPI>, W4<4>::LDS);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((ns_gemm_128<EPI>), dim3((unsigned)grid), dim3(256), lds, s, p);
+    hipLaunchKernelGGL((ns_gemm_128<EPI>), g, dim3(256), W4<4>::LDS, s, p);
   }
   return hipGetLastError();
 }
@@ -721,6 +747,8 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
 template <int KIND, int LAST>
 static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float eps, char* ws, hipStream_t s) {
   const bool tall = in.R > in.C;
+  // near-square matrices: single steps cost no more (7.5 n / m + 2.5 against 3 n / m + 7 products) and are more exact
+  if (5L * max(in.R, in.C) <= 7L * min(in.R, in.C)) seg = 1;
   NsSpace w = ns_space(ws, B, in.R, in.C, steps > seg);
   const int mp = (int)w.mp, np = (int)w.np;
   const int Rp = tall ? np : mp, Cp = tall ? mp : np;
@@ -783,7 +811,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
       ap.A = a; ap.lda = mp; ap.pa = tall ? w.px : w.ps; ap.ba = 2 * ap.pa;
       ap.B = b; ap.ldb = mp; ap.pb = tall ? w.ps : w.px; ap.bb = 2 * ap.pb;
       ap.M = Rp; ap.N = Cp; ap.K = mp; ap.cs = e2(-sq - SX);
-      ap.R = in.R; ap.Cc = in.C;
+      ap.R = in.R; ap.Cc = in.C; ap.il = in.il; ap.nb = in.B;
       ap.vec = in.C % 8 == 0 && (uintptr_t)ap.C % 16 == 0 && (uintptr_t)ap.w % 16 == 0 && (uintptr_t)ap.copy % 16 == 0 &&
                (uintptr_t)ap.lo % 16 == 0;
       NS_TRY(ns_launch<LAST>(ap, B, s));
@@ -811,21 +839,22 @@ int dllm_orthogonalize(const void* x, int xdt, void* out, int odt, int B, int R,
   const long need = dllm_muon_workspace(B, R, C, steps);
   if (need == 0 || ws == nullptr || ws_bytes < need || (uintptr_t)ws % 256) return -1;
   if ((xdt != DT_BF16 && xdt != DT_F32) || (odt != DT_BF16 && odt != DT_F32) || !x || !out) return -1;
-  MuonIn in{x, xdt, nullptr, 0.f, 1.f, 0, R, C};
+  MuonIn in{x, xdt, nullptr, 0.f, 1.f, 0, R, C, 0, B};
   NsGemm fin = {};
   fin.C = out; fin.cdt = odt;
   return ns_run<NS_ORTH, NS_OUT>(in, fin, B, steps, odt == DT_F32 ? 1 : NS_SEGMENT, eps, (char*)ws, (hipStream_t)stream);
 }
 
 // momentum update, orthogonalisation and W <- decay W - rate O, on an fp32 master (w, optional bf16 copy) or a split one
-// (lo, copy); gradient [B][R][C] bf16 / fp32, momentum fp32
+// (lo, copy); gradient [B][R][C] bf16 / fp32, momentum fp32.  il > 0: the matrices' rows alternate in blocks of il
 int dllm_muon_step(const void* g, int gdt, float* mom, float* w, void* copy, void* lo, int B, int R, int C, int steps,
-                   float eps, float beta, int nesterov, float gscale, float decay, float rate, void* ws, long ws_bytes,
-                   void* stream) {
+                   float eps, float beta, int nesterov, float gscale, float decay, float rate, int il, void* ws,
+                   long ws_bytes, void* stream) {
+  if (il < 0 || (il > 0 && R % il)) return -1;
   const long need = dllm_muon_workspace(B, R, C, steps);
   if (need == 0 || ws == nullptr || ws_bytes < need || (uintptr_t)ws % 256) return -1;
   if ((gdt != DT_BF16 && gdt != DT_F32) || !g || !mom || (!w && !(lo && copy)) || (w && lo)) return -1;
-  MuonIn in{g, gdt, mom, beta, gscale, nesterov, R, C};
+  MuonIn in{g, gdt, mom, beta, gscale, nesterov, R, C, il, B};
   NsGemm fin = {};
   fin.w = w; fin.copy = (uint16_t*)copy; fin.lo = (int16_t*)lo; fin.decay = decay; fin.rate = rate;
   return ns_run<NS_MUON, NS_STEP>(in, fin, B, steps, NS_SEGMENT, eps, (char*)ws, (hipStream_t)stream);

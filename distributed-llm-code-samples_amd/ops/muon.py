@@ -100,7 +100,13 @@ def muon_scale(rows: int, cols: int) -> float:
     return math.sqrt(max(1.0, rows / cols))
 
 
-def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, master, copy, lo) -> None:
+def _blocks_of(t: torch.Tensor, interleave: int) -> torch.Tensor:
+    """[2, R, C] view-or-copy of the two matrices whose rows alternate in blocks of ``interleave``."""
+    C = t.shape[1]
+    return t.view(-1, 2, interleave, C).transpose(0, 1).reshape(2, -1, C)
+
+
+def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, interleave, master, copy, lo) -> None:
     ref = lo if master is None else master
     B, R, C = _dims(ref, "the weight")
     _check_steps(steps)
@@ -109,6 +115,11 @@ def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale,
     _check_dense(momentum, "momentum", ref.shape, (torch.float32,), ref.device)
     if copy is not None:
         _check_dense(copy, "the bf16 copy", ref.shape, (torch.bfloat16,), ref.device)
+    if interleave:
+        if ref.dim() != 2 or interleave < 0 or R % (2 * interleave):
+            raise ValueError(f"interleave = {interleave} needs a 2-D weight with rows in multiples of {2 * abs(interleave)}, "
+                             f"got {tuple(ref.shape)}")
+        B, R = 2, R // 2
     if ref.numel() == 0:
         return
     rate = lr * (muon_scale(R, C) if scale is None else scale)
@@ -116,7 +127,12 @@ def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale,
     if ref.device.type != "cuda":
         g = grad.float() * grad_scale
         momentum.mul_(beta).add_(g)
-        o = _newton_schulz_torch(g + beta * momentum if nesterov else momentum, steps, eps)
+        u = g + beta * momentum if nesterov else momentum
+        if interleave:
+            o = _newton_schulz_torch(_blocks_of(u, interleave), steps, eps)
+            o = o.view(2, -1, interleave, C).transpose(0, 1).reshape(u.shape)
+        else:
+            o = _newton_schulz_torch(u, steps, eps)
         if master is not None:
             master.mul_(decay).sub_(rate * o)
             if copy is not None:
@@ -129,28 +145,32 @@ def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale,
         ws = _workspace(B, R, C, steps, ref.device)
         rc = _native.lib().dllm_muon_step(grad.data_ptr(), _native.dtype_code(grad.dtype), momentum.data_ptr(), ptr(master),
                                           ptr(copy), ptr(lo), B, R, C, steps, float(eps), float(beta), int(nesterov),
-                                          float(grad_scale), float(decay), float(rate), ws.data_ptr(), ws.numel(),
-                                          _native.stream_ptr(ref.device))
-    _native.check(rc, f"dllm_muon_step({B}x{R}x{C})")
+                                          float(grad_scale), float(decay), float(rate), int(interleave), ws.data_ptr(),
+                                          ws.numel(), _native.stream_ptr(ref.device))
+    if rc:
+        _native.check(rc, f"dllm_muon_step({B}x{R}x{C})")
 
 
 def muon_step_(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, lr: float, beta: float = 0.95,
                nesterov: bool = True, wd: float = 0.0, steps: int = NS_STEPS, eps: float = NS_EPS,
-               copy: torch.Tensor | None = None, scale: float | None = None, grad_scale: float = 1.0) -> None:
+               copy: torch.Tensor | None = None, scale: float | None = None, grad_scale: float = 1.0,
+               interleave: int = 0) -> None:
     """Muon on fp32 weights ``master`` [R, C] (or a batch [B, R, C] of equal shape, each its own matrix), in place:
 
     ``momentum = beta·momentum + g``, ``U = g + beta·momentum`` (``nesterov``) or ``momentum``, ``O = orthogonalize(U)``,
     ``master = (1 - lr·wd)·master - lr·scale·O``, ``copy = bf16(master)``,  with ``g = grad_scale·grad`` (bf16 or fp32).
-    ``scale`` defaults to ``muon_scale(R, C)``."""
+    ``scale`` defaults to ``muon_scale(R, C)``.  ``interleave``: ``master`` [2 R, C] holds two matrices whose rows alternate
+    in blocks of that many (the gated FFN's W13), each stepped as its own."""
     if master.dtype != torch.float32:
         raise TypeError("master weights must be fp32")
-    _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, master, copy, None)
+    _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, interleave, master, copy, None)
 
 
 def muon_split_step_(lo: torch.Tensor, hi: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, lr: float,
                      beta: float = 0.95, nesterov: bool = True, wd: float = 0.0, steps: int = NS_STEPS,
-                     eps: float = NS_EPS, scale: float | None = None, grad_scale: float = 1.0) -> None:
+                     eps: float = NS_EPS, scale: float | None = None, grad_scale: float = 1.0,
+                     interleave: int = 0) -> None:
     """``muon_step_`` on a split master (``ops/master.py``): ``lo`` the int16 residual plane, ``hi`` the bf16 working copy."""
     if lo.dtype != torch.int16 or hi.dtype != torch.bfloat16 or lo.shape != hi.shape:
         raise TypeError("muon_split_step_ takes an int16 residual plane and its bf16 working copy")
-    _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, None, hi, lo)
+    _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, interleave, None, hi, lo)
