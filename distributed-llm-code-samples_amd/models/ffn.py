@@ -26,6 +26,7 @@ from typing import NamedTuple
 
 import torch
 
+from ..ops.fp8 import BlockFP8, gemm_fp8, quantize_fp8, quantize_fp8_both, quantize_fp8_t
 from ..ops.gemm import gemm, gemm_pair
 from ..utils.config import INIT_SCALE
 
@@ -215,6 +216,59 @@ def layer_bwd(dy: torch.Tensor, x: torch.Tensor, w1: torch.Tensor, w2: torch.Ten
         if hooks is not None:
             hooks.after_dx(dx)
     wgrad_w1(da_buf, x, kw1, nn)                                      # dW1 = daᵀ·x        [F, D]
+    if hooks is not None:
+        hooks.after_w1()
+    return dx
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# 8-bit layer (TrainConfig.fp8): the reference layer's six products (train_ffns.py:54-70) on block-scaled operands
+# (ops/fp8.py).  Activations and weights are e4m3, output gradients e5m2; x, a and their gradients are quantised once each,
+# both ways in one read (rows for the forward / input-gradient product, columns for the weight gradient); weights per
+# 128x128 tile, transposed anew in the backward (one more read, no second copy kept).  Activations stay in the compute dtype
+# between the products, and the weight gradients have their buffers' type (fp32 buffers: exact products, fp32 sums).
+# ------------------------------------------------------------------------------------------------------------------
+class FP8Saved(NamedTuple):
+    """The forward's 8-bit weight-gradient operands of one layer: xᵀ [D, T] and aᵀ [F, T]."""
+    x_t: BlockFP8
+    a_t: BlockFP8
+
+
+def layer_fwd_fp8(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, act: str, a_out: torch.Tensor,
+                  h_out: torch.Tensor | None, y_out: torch.Tensor, before_fwd2=None) -> FP8Saved:
+    """``y = act(x·W1ᵀ)·W2ᵀ`` on 8-bit operands; ``a_out`` / ``h_out`` as in ``layer_fwd``."""
+    xq, x_t = quantize_fp8_both(x)
+    gemm_fp8(xq, quantize_fp8(w1, tile=True), a_out, epi="act", act=act, aux_out=h_out)
+    aq, a_t = quantize_fp8_both(a_out)
+    if before_fwd2 is not None:
+        before_fwd2()
+    gemm_fp8(aq, quantize_fp8(w2, tile=True), y_out)
+    return FP8Saved(x_t, a_t)
+
+
+def layer_bwd_fp8(dy: torch.Tensor, saved: FP8Saved, w1: torch.Tensor, w2: torch.Tensor, act: str, a: torch.Tensor,
+                  h: torch.Tensor | None, gw1: torch.Tensor, gw2: torch.Tensor, da_buf: torch.Tensor,
+                  dx_out: torch.Tensor | None, hooks=None) -> torch.Tensor | None:
+    """Backward of ``layer_fwd_fp8`` into the gradient tensors ``gw1`` / ``gw2``; returns dx.  Order as ``layer_bwd``
+    (``da, dW2, dx, dW1``; without dx ``da, dW1, dW2``)."""
+    dyq, dy_t = quantize_fp8_both(dy, "e5m2", "e5m2")
+    gemm_fp8(dyq, quantize_fp8_t(w2, tile=True), da_buf, epi="dact", act=act, aux=h if h is not None else a)
+    if dx_out is None:
+        gemm_fp8(quantize_fp8_t(da_buf, "e5m2"), saved.x_t, gw1)
+        if hooks is not None:
+            hooks.after_w1()
+        gemm_fp8(dy_t, saved.a_t, gw2)
+        if hooks is not None:
+            hooks.after_w2()
+        return None
+    gemm_fp8(dy_t, saved.a_t, gw2)
+    if hooks is not None:
+        hooks.after_w2()
+    daq, da_t = quantize_fp8_both(da_buf, "e5m2", "e5m2")
+    dx = gemm_fp8(daq, quantize_fp8_t(w1, tile=True), dx_out)
+    if hooks is not None:
+        hooks.after_dx(dx)
+    gemm_fp8(da_t, saved.x_t, gw1)
     if hooks is not None:
         hooks.after_w1()
     return dx

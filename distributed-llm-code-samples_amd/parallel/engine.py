@@ -44,10 +44,11 @@ from dataclasses import dataclass
 
 import torch
 
-from ..models.ffn import (NNWgrad, deinterleave_w13, interleave_w13, layer_bwd, layer_bwd_t, layer_fwd, layer_fwd_t,
-                          needs_preact, recompute_fwd1, wgrad_w1, wgrad_w2)
+from ..models.ffn import (GLU_BLOCK, NNWgrad, deinterleave_w13, interleave_w13, layer_bwd, layer_bwd_fp8, layer_bwd_t,
+                          layer_fwd, layer_fwd_fp8, layer_fwd_t, needs_preact, recompute_fwd1, wgrad_w1, wgrad_w2)
 from ..ops.elementwise import adam_split_step_, adam_step_, cast_, sgd_split_step_, sgd_step_
 from ..ops.master import join_flat, part_flat
+from ..ops.muon import muon_scale, muon_split_step_, muon_step_
 from ..utils import streams
 from ..utils.config import TrainConfig
 from . import comm
@@ -178,7 +179,7 @@ class FFNTrainer:
         # activations [F, T], W2 stored as W2ᵀ [F, D]
         from ..ops.gemm import use_m224
 
-        self.tmode = (cfg.tp_transposed and self.device.type == "cuda" and not self.gated and not self.fsdp
+        self.tmode = (cfg.tp_transposed and not cfg.fp8 and self.device.type == "cuda" and not self.gated and not self.fsdp
                       and not self.zero and not self.sp and cfg.recompute == "none" and self.cd == torch.bfloat16
                       and use_m224(self.F_loc, T) and use_m224(self.F_loc, D) and T % 256 == 0)
         self.step_count = 0
@@ -195,6 +196,23 @@ class FFNTrainer:
             # with one: hybrid 172.2-172.4 vs 175.8-176.1 ms, zero 30.5-30.7 vs 30.9-31.0
             # (profiles/r4/min_bpc_forcecomm_r4.txt)
             set_min_blocks_per_cu(cfg.gemm_min_bpc or (2 if mesh.world > 1 else 1))
+
+        if cfg.optimizer not in ("sgd", "adam", "muon"):
+            raise ValueError(f"unknown optimizer {cfg.optimizer!r}: expected sgd | adam | muon")
+        self.muon = cfg.optimizer == "muon"
+        if self.muon and (self.zero or self.fsdp or t > 1):
+            # the update is a function of the whole matrix: a rank must hold it and its full gradient
+            raise ValueError("optimizer muon needs whole weight matrices on every rank: single device or dp_mode ddp "
+                             "(no ZeRO / FSDP shards, no tensor parallelism)")
+        self.fp8 = cfg.fp8
+        if self.fp8:
+            bad = [why for cond, why in ((self.cd != torch.bfloat16, "dtype bf16"), (self.gated, "an ungated FFN"),
+                                         (self.tp_comm or t > 1, "no tensor parallelism"),
+                                         (cfg.recompute != "none", "recompute none"),
+                                         (cfg.w2_storage == "transposed", "W2 row-major"),
+                                         (cfg.wgrad_layout in ("nn", "nn_w1", "nn_w2t"), "wgrad_layout auto or tn")) if cond]
+            if bad:
+                raise ValueError("fp8 needs " + ", ".join(bad))
 
         if cfg.debug_sync:
             comm.set_serialize(True)
@@ -241,12 +259,14 @@ class FFNTrainer:
                       and not (self.side_opt and cfg.side_optimizer > 0))   # the capped SGD kernel: fp32 masters
         if cfg.master not in ("split", "fp32"):
             raise ValueError(f"unknown master format {cfg.master!r}")
-        self.fused_opt = cfg.fused_optimizer and no_coll and not self.side_opt
+        # (muon and the 8-bit layers store their gradients: muon's update needs the whole one, their products have no
+        # optimizer epilogue)
+        self.fused_opt = cfg.fused_optimizer and no_coll and not self.side_opt and not self.muon and not self.fp8
         # grouped weight-gradient pair (small tile grids: the MP / TP8 shard's dW2 [D, F/8] and dW1 [F/8, D] would each
         # run split-K plus a reduction pass): both in one launch of whole tiles, after dx (models/ffn.layer_bwd).  It
         # replaces the weight-gradient stream there: two part-empty grids have no tail worth filling
         self.pair_wgrads = False
-        if dev.type == "cuda" and not self.tmode:
+        if dev.type == "cuda" and not self.tmode and not self.fp8:
             from ..ops.gemm import pair_supported
 
             self.pair_wgrads = pair_supported(((D, self.F_loc, T), (self.R1, D, T)), self.cd)
@@ -352,6 +372,8 @@ class FFNTrainer:
         if cfg.optimizer == "adam":
             self.adam_m = torch.zeros(nmaster, dtype=torch.float32, device=dev)
             self.adam_v = torch.zeros(nmaster, dtype=torch.float32, device=dev)
+        if self.muon:
+            self.muon_m = torch.zeros(nmaster, dtype=torch.float32, device=dev)
 
         # ---- FSDP rings --------------------------------------------------------------------------
         if self.fsdp:
@@ -376,6 +398,7 @@ class FFNTrainer:
         Tl = T // t if self.sp else T  # tokens held per rank between layers
         self.Tl = Tl
         car_arena = self.tp_car is not None and self.tp_car.arena is not None
+        self.fp8_saved = [None] * L   # 8-bit layers: the forward's weight-gradient operands, until the layer's backward
         self.xs = [None] + [self.tp_car.arena_view((Tl, D), self.cd) if car_arena else
                             torch.empty((Tl, D), dtype=self.cd, device=dev) for _ in range(L)]
         keep = cfg.recompute == "none"
@@ -389,7 +412,7 @@ class FFNTrainer:
         self.da = torch.empty(hsh, dtype=self.cd, device=dev)
         # ReLU: 1-bit activation-gradient masks (written by the forward's first GEMM, read by the dgrad)
         self.masks = None
-        if cfg.relu_mask and self.act == "relu" and not self.gated and dev.type == "cuda":
+        if cfg.relu_mask and self.act == "relu" and not self.gated and not self.fp8 and dev.type == "cuda":
             from ..ops.gemm import relu_mask_bytes, relu_mask_supported
 
             mM, mN = (self.F_loc, T) if self.tmode else (T, self.F_loc)
@@ -521,7 +544,7 @@ class FFNTrainer:
         cfg = self.cfg
         if cfg.wgrad_layout not in ("auto", "tn", "nn", "nn_w1", "nn_w2t"):
             raise ValueError(f"unknown wgrad_layout {cfg.wgrad_layout!r}")
-        if cfg.wgrad_layout == "tn":
+        if cfg.wgrad_layout == "tn" or cfg.fp8:
             return False
         from ..ops.gemm import _VARIANT, BF16_VARIANTS
 
@@ -728,6 +751,8 @@ class FFNTrainer:
             self._master_stage = out["params"]
         if self.cfg.optimizer == "adam":
             out["adam_m"], out["adam_v"] = self.adam_m, self.adam_v
+        if self.muon:
+            out["muon_m"] = self.muon_m
         return out
 
     @torch.no_grad()
@@ -916,8 +941,30 @@ class FFNTrainer:
                       opt_m=self._view(self.adam_m, e), opt_v=self._view(self.adam_v, e))
         return kw
 
+    def _opt_muon(self, s: int, e: int) -> None:
+        """Muon on the weights in flat range [s, e) (whole entries: ranges are entries, buckets or everything).  W13 is its
+        two matrices, W2ᵀ storage changes nothing but the logical shape that sets the update's scale."""
+        cfg = self.cfg
+        for en in self.entries:
+            if not s <= en.offset < e:
+                continue
+            rows, cols = en.shape
+            il = GLU_BLOCK if self.gated and en.name == "w1" else 0
+            lr_, lc = (cols, rows) if self.w2t and en.name == "w2" else (rows // 2 if il else rows, cols)
+            v = lambda flat: self._view(flat, en)  # noqa: E731
+            kw = {"lr": cfg.lr, "beta": cfg.muon_beta, "nesterov": cfg.muon_nesterov, "wd": cfg.weight_decay,
+                  "scale": muon_scale(lr_, lc), "interleave": il}
+            if self.split:
+                muon_split_step_(v(self.master_lo), v(self.copy), v(self.grads), v(self.muon_m), **kw)
+            else:
+                muon_step_(v(self._master), v(self.grads), v(self.muon_m), copy=None if self.shared_copy else v(self.copy),
+                           **kw)
+
     def _opt(self, s: int, e: int) -> None:
         cfg = self.cfg
+        if self.muon:
+            self._opt_muon(s, e)
+            return
         if self.split:  # full or FSDP-shard layout: the residual plane shares the working copy's offsets
             if cfg.optimizer == "sgd":
                 sgd_split_step_(self.master_lo[s:e], self.copy[s:e], self.grads[s:e], cfg.lr)
@@ -1247,6 +1294,8 @@ class FFNTrainer:
                     continue
                 if self.tmode:
                     layer_fwd_t(self.xs[l], w1, w2, act, a, h, self.xs[l + 1], before_fwd2=before2, mask=self._mask(l))
+                elif self.fp8:
+                    self.fp8_saved[l] = layer_fwd_fp8(self.xs[l], w1, w2, act, a, h, self.xs[l + 1], before_fwd2=before2)
                 else:
                     layer_fwd(self.xs[l], w1, w2, act, gated, a, h, self.xs[l + 1], before_fwd2=before2,
                               mask=self._mask(l), y_t=self.xT[l + 1] if self.wgrad_nn and l + 1 < L else None,
@@ -1331,6 +1380,12 @@ class FFNTrainer:
             elif self.tmode:
                 dx = layer_bwd_t(g, self.xs[l], w1, w2, act, a, h, gw1, gw2, self.da,
                                  self.dxb[l % 2] if need_dx else None, hooks, mask=self._mask(l))
+                if dx is not None:
+                    g = dx
+            elif self.fp8:
+                saved, self.fp8_saved[l] = self.fp8_saved[l], None
+                dx = layer_bwd_fp8(g, saved, w1, w2, act, a, h, gw1, gw2, self.da, self.dxb[l % 2] if need_dx else None,
+                                   hooks)
                 if dx is not None:
                     g = dx
             else:

@@ -42,6 +42,7 @@ def config_from_args(a) -> TrainConfig:
     return TrainConfig(model=m, batch_size=a.batch_size, seq_len=a.seq_len, num_steps=a.num_steps,
                        random_seed=a.random_seed, dtype=a.dtype, grad_dtype=a.grad_dtype or a.dtype,
                        optimizer=a.optimizer, lr=a.lr, weight_decay=a.weight_decay,
+                       muon_beta=a.muon_beta, fp8=a.fp8,
                        sequence_parallel=a.sequence_parallel, recompute=a.recompute, bucket_mb=a.bucket_mb,
                        data=a.data, comm_backend=a.comm, debug_sync=a.debug_sync, tp_allreduce=a.tp_allreduce, wgrad_layout=a.wgrad_layout,
                        w2_storage=a.w2_storage,

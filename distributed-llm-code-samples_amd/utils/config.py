@@ -48,12 +48,17 @@ class TrainConfig:
     random_seed: int = 0             # -r (0 = unseeded, train_ffns.py:355-358)
     dtype: str = "fp32"              # compute dtype: fp32 (reference parity) | bf16
     grad_dtype: str = "fp32"         # dtype of gradients / gradient collectives
-    optimizer: str = "sgd"           # sgd (reference) | adam
+    optimizer: str = "sgd"           # sgd (reference) | adam | muon (ops/muon.py: momentum, orthogonalised update)
     lr: float = LR
     adam_b1: float = 0.9
     adam_b2: float = 0.95
     adam_eps: float = 1e-8
     weight_decay: float = 0.0
+    muon_beta: float = 0.95
+    muon_nesterov: bool = True
+    # bf16 runs: the layers' six products on 8-bit operands (ops/fp8.py): activations and weights e4m3, gradients e5m2,
+    # scaled per 128 (weights: 128x128); activations, gradients and masters keep their types
+    fp8: bool = False
     dp_mode: str = "none"            # none | ddp | zero (ZeRO-2: sharded optimizer) | fsdp (ZeRO-3)
     dp: int = 1
     tp: int = 1
@@ -146,7 +151,10 @@ def add_extended_args(p: argparse.ArgumentParser) -> None:
     p.add_argument("--act", choices=["relu", "silu", "gelu"], default="relu")
     p.add_argument("--ffn_dim", type=int, default=0)
     p.add_argument("--gated", action="store_true")
-    p.add_argument("--optimizer", choices=["sgd", "adam"], default="sgd")
+    p.add_argument("--optimizer", choices=["sgd", "adam", "muon"], default="sgd")
+    p.add_argument("--muon_beta", type=float, default=0.95, help="momentum of --optimizer muon")
+    p.add_argument("--fp8", action="store_true",
+                   help="8-bit products with a scale per block of 128 (needs --dtype bf16, no --gated, no tensor parallelism)")
     p.add_argument("--lr", type=float, default=LR)
     p.add_argument("--weight_decay", type=float, default=0.0)
     p.add_argument("--backend", choices=["auto", "nccl", "rccl", "gloo"], default="auto")

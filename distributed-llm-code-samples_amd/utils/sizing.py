@@ -42,7 +42,7 @@ def plan(D: int, F: int, L: int, tokens: int, dp: int = 1, tp: int = 1, mode: st
          act: str = "relu", dtype: str = "bf16", grad_dtype: str = "bf16", optimizer: str = "sgd",
          recompute: str = "none", relu_mask: bool = True, sequence_parallel: bool = False,
          align: int = 64, wgrad_stream: bool = False, master: str = "split", wgrad_layout: str = "auto",
-         on_gpu: bool = True) -> dict:
+         on_gpu: bool = True, fp8: bool = False) -> dict:
     """Per-rank bytes by buffer (and GiB totals).  ``mode``: none | ddp | zero | fsdp (over ``dp`` ranks).
     ``wgrad_stream``: the concurrent weight-gradient stream (single device, fused optimizer, kept activations, no
     TP) rotates two dgrad and three dx buffers instead of one and two (``FFNTrainer.da_ring`` / ``dxb``).
@@ -51,7 +51,9 @@ def plan(D: int, F: int, L: int, tokens: int, dp: int = 1, tp: int = 1, mode: st
     ``wgrad_layout`` (the engine's resolved mode, ``FFNTrainer.wgrad_nn`` / ``wgrad_nn_w2``): nn_w1 keeps a transposed
     copy xᵀ [D, T] of every layer input, nn / nn_w2t also dyᵀ copies rotating with the dx buffers plus the top layer's;
     the NN modes run the backward serially (no weight-gradient stream).  "auto" resolves as the engine does
-    (``resolve_wgrad_layout``): nn_w2t on a GPU wherever the layout runs, else tn."""
+    (``resolve_wgrad_layout``): nn_w2t on a GPU wherever the layout runs, else tn.
+    ``fp8``: the 8-bit layers keep xᵀ and aᵀ in 8 bits (and their scales) until the backward; stored gradients, no ReLU
+    masks, no transposed copies (the quantised operands of one product at a time are transients, not counted)."""
     cd = 2 if dtype == "bf16" else 4
     gd = 2 if grad_dtype == "bf16" else 4
     multi = dp > 1
@@ -69,10 +71,12 @@ def plan(D: int, F: int, L: int, tokens: int, dp: int = 1, tp: int = 1, mode: st
         b["master_fp32"] = master_n * 4
     shared_copy = cd == 4 and not zero
     b["compute_copy"] = 0 if shared_copy else total * cd
-    fused = not (ddp or zero or fsdp)
+    fused = not (ddp or zero or fsdp) and optimizer != "muon" and not fp8
     b["grads"] = 0 if fused else total * gd
     if optimizer == "adam":
         b["adam_moments"] = 2 * master_n * 4
+    if optimizer == "muon":
+        b["muon_momentum"] = master_n * 4
     if zero:
         b["zero_grad_shard"] = (total // dp) * gd
     if fsdp:
@@ -89,7 +93,10 @@ def plan(D: int, F: int, L: int, tokens: int, dp: int = 1, tp: int = 1, mode: st
     b["activations"] = nA * T * F_loc * cd
     if need_h:
         b["preactivations"] = nA * T * R1 * cd
-    if relu_mask and act == "relu" and not gated and dtype == "bf16":
+    if fp8:
+        wgrad_layout = "tn"
+        b["fp8_saved"] = L * (T * D + T * F_loc) * 129 // 128
+    if relu_mask and act == "relu" and not gated and dtype == "bf16" and not fp8:
         b["relu_masks"] = nA * (T // 256) * (F_loc // 256) * 8192
     wgrad_layout = resolve_wgrad_layout(wgrad_layout, D, F_loc, R1, T, mode=mode if multi else "none", tp=tp,
                                         dtype=dtype, recompute=recompute, sp=sp, master=master, on_gpu=on_gpu)
@@ -103,7 +110,7 @@ def plan(D: int, F: int, L: int, tokens: int, dp: int = 1, tp: int = 1, mode: st
         b["nn_transposed_copies"] = (L + (3 if wgrad_layout != "nn_w1" else 0)) * D * T * cd
     if sp:
         b["sp_buffers"] = (3 + (L if keep else 0)) * T * D * cd + 2 * Tl * D * cd
-    state = sum(v for k, v in b.items() if k in ("master_fp32", "master_residual", "compute_copy", "grads", "adam_moments",
+    state = sum(v for k, v in b.items() if k in ("master_fp32", "master_residual", "compute_copy", "grads", "adam_moments", "muon_momentum",
                                                    "zero_grad_shard", "fsdp_weight_ring", "fsdp_grad_ring"))
     tot = sum(b.values())
     g = 2**30
