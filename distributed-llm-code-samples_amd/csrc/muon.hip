@@ -574,7 +574,8 @@ __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) 
     const int fs = slot;
     slot = slot + 1 == W::STAGES ? 0 : slot + 1;
     const uint32_t off = (uint32_t)(slot * W::STAGE);
-    constexpr int PR = F / 2 - (F < 6);            // matrix instructions per read (0, 1, 2), then two per fetch
+    constexpr int PR = F / 2 - 1;                  // matrix instructions per read (0, 1, 2), then two per fetch
+    static_assert(4 * F * PR + 2 * F * 2 == 2 * F * F, "every matrix instruction of the step, once");
     upto(NR{}, [&](auto j) {
       read(other, j, off);
       __builtin_amdgcn_sched_barrier(0);

@@ -156,3 +156,17 @@ def test_other_stream_and_graph():
         muon.muon_step_(we, gn, me, lr=0.02)
         torch.cuda.synchronize()
         assert torch.equal(w, we) and torch.equal(m, me)
+
+
+@pytest.mark.parametrize("R,C", [(4096, 4224), (8192, 4096), (2900, 3100), (1024, 8200), (2048, 2048), (1300, 1300)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_orthogonalize_large(R, C, out):
+    """Sizes that take the larger tiles, against the iteration in 64 bits; memory that the workspace may get holds NaN."""
+    x = gradient(R, C, R + C).to(DEV)
+    ref = muon._newton_schulz_torch(x.double(), 5, muon.NS_EPS)
+    err = lambda t: (torch.linalg.norm(t.double() - ref) / torch.linalg.norm(ref)).item()  # noqa: E731
+    tol = 4 * err(muon._newton_schulz_torch(x, 5, muon.NS_EPS)) + 8 * 2.0 ** -23 + (2.0 ** -8 if out == torch.bfloat16 else 0.0)
+    fill = torch.full((1 << 29,), float("nan"), device=DEV)
+    del fill
+    got = muon.orthogonalize(x, out=torch.empty(R, C, dtype=out, device=DEV))
+    assert err(got) <= tol
