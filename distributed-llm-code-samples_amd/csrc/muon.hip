@@ -302,6 +302,10 @@ __device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n,
   }
 }
 
+static void ns_set_vec(NsGemm& p) {
+  p.vec = p.Cc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.copy % 16 == 0 && (uintptr_t)p.lo % 16 == 0;
+}
+
 // 256x256 tiles on the 8-phase loop (nt8.h): the three plane pairs as one run of 3 K / 64 K steps
 struct NsTrait {
   const char *a, *b;
@@ -744,9 +748,331 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
     if (err_ != hipSuccess) return (int)err_;     \
   } while (0)
 
+// ----------------------------------------------------------------------------------------------
+// shorter side m <= 128: one launch per step
+//
+// A and P (128 x 128, padded with zeros) fit a block, so every block computes P for itself and applies it to its own columns
+// of X, then leaves its part of the next A, the fp32 Gram matrix of the columns it just wrote; the next launch adds the
+// parts up in their order.  Launches and their latency bound it: 300 x 101, five steps, 17 launches of the kernels above
+// take 87 us.
+//
+// X lives in operand order, "fragments": chunk (nt, kk) of a plane is 64 lanes x 8 values, lane (g, i) = (lane / 16,
+// lane % 16) holding column 16 nt + i, rows 32 kk + 4 g + (0 .. 3) and 32 kk + 16 + 4 g + (0 .. 3).  That is what a lane has
+// of two neighbouring results of the matrix instruction, so results become operands without leaving their lane; the order
+// of rows inside a chunk is the same in both operands of every product, and the sum does not see it.
+// Wave (rw, cw) owns rows 32 rw .. 32 rw + 31 and columns 32 cw .. 32 cw + 31 of A and P, 16 cw .. 16 cw + 15 of a slice.
+// ----------------------------------------------------------------------------------------------
+constexpr int NS_SMALL = 128;
+constexpr int SM_SLICE = 64;          // columns of X at a time
+constexpr int SM_BLOCKS = 256;        // blocks (parts of A) per matrix, at most
+constexpr int SM_DIRECT = 8;          // parts that a step adds up by itself; more are added by a launch of their own
+constexpr int SM_TLD = NS_SMALL + 4;  // LDS row of a slice in fp32
+constexpr int SM_PART = NS_SMALL * NS_SMALL;
+
+struct NsSmall {
+  MuonIn in;
+  const double* part;
+  float eps;
+  f16* X; long px;                    // fragment planes; px: elements of a plane; matrices 2 px apart
+  const float* gin; int parts;        // parts of A to add, [matrix][parts][SM_PART], as the waves hold them
+  float* gout;                        // [matrix][gridDim.x][SM_PART]
+  int m, n, slices, tall;
+};
+
+struct SmFrag { f16x8_t h, l; };
+__device__ __forceinline__ SmFrag sm_frag(const f32x4_t& a, const f32x4_t& b, float s) {
+  SmFrag f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    f16 hh, ll;
+    split16((e < 4 ? a[e] : b[e - 4]) * s, hh, ll);
+    f.h[e] = hh;
+    f.l[e] = ll;
+  }
+  return f;
+}
+// One of the four plane products of rows of a (4 g + r) and rows of b (i): lo lo, lo hi, hi lo into d, hi hi into c.  lo lo
+// too: in a sum of few terms its 2^-22 does not average out, and five steps on one number end at 4.4e-7 (median) without it,
+// 3.6e-7 with it and in fp32.  Callers run one product of four results before the next: one after the other on the same sum
+// would wait for each (twice the time).
+template <int S>
+__device__ __forceinline__ void sm_mma(f32x4_t& c, f32x4_t& d, const SmFrag& a, const SmFrag& b) {
+  f32x4_t& s = S == 3 ? c : d;
+  s = __builtin_amdgcn_mfma_f32_16x16x32_f16(S & 2 ? a.h : a.l, S & 1 ? b.h : b.l, s, 0, 0, 0);
+}
+template <class F> __device__ __forceinline__ void sm_each(F f) {
+  f(std::integral_constant<int, 0>{});
+  f(std::integral_constant<int, 1>{});
+  f(std::integral_constant<int, 2>{});
+  f(std::integral_constant<int, 3>{});
+}
+__device__ __forceinline__ void sm_put(f16x8_t* base, int chunks, int c, int lane, const SmFrag& f) {
+  base[c * 64 + lane] = f.h;
+  base[(chunks + c) * 64 + lane] = f.l;
+}
+__device__ __forceinline__ SmFrag sm_get(const f16x8_t* base, int chunks, int c, int lane) {
+  return SmFrag{base[c * 64 + lane], base[(chunks + c) * 64 + lane]};
+}
+// this wave's part of the Gram matrix of a slice whose fragments are in LDS, chunk nk * 8 + mt
+__device__ __forceinline__ void sm_gram(const f16x8_t* gf, int rw, int cw, int lane, f32x4_t (&c)[2][2], f32x4_t (&d)[2][2]) {
+#pragma unroll
+  for (int nk = 0; nk < 2; ++nk) {
+    const SmFrag a[2] = {sm_get(gf, 16, nk * 8 + 2 * rw, lane), sm_get(gf, 16, nk * 8 + 2 * rw + 1, lane)};
+    const SmFrag b[2] = {sm_get(gf, 16, nk * 8 + 2 * cw, lane), sm_get(gf, 16, nk * 8 + 2 * cw + 1, lane)};
+    sm_each([&](auto s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sm_mma<s.value>(c[i >> 1][i & 1], d[i >> 1][i & 1], b[i & 1], a[i >> 1]);
+    });
+  }
+}
+__device__ __forceinline__ void sm_part_out(const NsSmall& p, int rw, int cw, int lane, const f32x4_t (&c)[2][2], const f32x4_t (&d)[2][2]) {
+  f32x4_t* o = (f32x4_t*)(p.gout + ((long)blockIdx.y * gridDim.x + blockIdx.x) * SM_PART);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[((2 * rw + (i >> 1)) * 8 + 2 * cw + (i & 1)) * 64 + lane] = c[i >> 1][i & 1] + d[i >> 1][i & 1];
+}
+__device__ __forceinline__ void sm_clear(f32x4_t (&c)[2][2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) (&c[0][0])[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+}
+
+// X_0 in fragments and its parts of A.  grid (blocks, matrices)
+template <int KIND>
+__global__ __launch_bounds__(1024) void ns_small_first(NsSmall p) {
+  __shared__ __attribute__((aligned(16))) float tile[SM_SLICE * SM_TLD];
+  __shared__ __attribute__((aligned(16))) f16x8_t gf[2 * 16 * 64];
+  __shared__ double red[4];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, rw = w & 3, cw = w >> 2, i15 = lane & 15, g = lane >> 4, z = blockIdx.y;
+  if (w < 4) {
+    double s = p.part[(long)z * NS_PARTS + t];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
+    if (lane == 0) red[w] = s;
+  }
+  __syncthreads();
+  const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3]));
+  const float inv = (float)((double)(1 << SX) / (norm + (double)p.eps));
+  f32x4_t c[2][2], d[2][2];
+  sm_clear(c);
+  sm_clear(d);
+  for (int sl = blockIdx.x; sl < p.slices; sl += gridDim.x) {
+    const int n0 = sl * SM_SLICE;
+#pragma unroll
+    for (int k = 0; k < SM_SLICE * NS_SMALL / 1024; ++k) {        // neighbouring threads along U's rows
+      const int j = t + 1024 * k, n = p.tall ? j >> 7 : j & 63, m = p.tall ? j & 127 : j >> 6;
+      float v = 0.f;
+      if (m < p.m && n0 + n < p.n) {
+        const int r = p.tall ? n0 + n : m, col = p.tall ? m : n0 + n;
+        v = muon_u<KIND>(p.in, muon_row(p.in.il, p.in.B, p.in.R, p.in.C, z, r) + col) * inv;
+      }
+      tile[n * SM_TLD + m] = v;
+    }
+    __syncthreads();
+    f16x8_t* x = (f16x8_t*)(p.X + (long)z * 2 * p.px);
+    const float* q = tile + (16 * cw + i15) * SM_TLD + 32 * rw + 4 * g;
+    sm_put(x, (int)(p.px >> 9), sl * 16 + cw * 4 + rw, lane, sm_frag(*(const f32x4_t*)q, *(const f32x4_t*)(q + 16), 1.f));
+    f32x4_t a, b;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      a[r] = tile[(32 * (w >> 3) + 4 * g + r) * SM_TLD + 16 * (w & 7) + i15];
+      b[r] = tile[(32 * (w >> 3) + 16 + 4 * g + r) * SM_TLD + 16 * (w & 7) + i15];
+    }
+    sm_put(gf, 16, w, lane, sm_frag(a, b, 1.f));
+    __syncthreads();
+    sm_gram(gf, rw, cw, lane, c, d);
+    __syncthreads();
+  }
+  sm_part_out(p, rw, cw, lane, c, d);
+}
+
+// parts of A added up in order: every fourth one per wave, then the four waves.  grid (64 results, matrices)
+__global__ __launch_bounds__(256) void ns_small_sum(const float* in, int parts, float* out) {
+  __shared__ f32x4_t red[4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const f32x4_t* q = (const f32x4_t*)(in + (long)blockIdx.y * parts * SM_PART) + blockIdx.x * 64 + lane;
+  f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = w; k < parts; k += 4) s += q[(long)k * (SM_PART / 4)];
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0)
+    ((f32x4_t*)(out + (long)blockIdx.y * SM_PART))[blockIdx.x * 64 + lane] = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+}
+
+// one step.  EPI NS_PLANES: X <- P X in place, and its parts of the next A; NS_OUT / NS_STEP: the result.  Sixteen waves of
+// little code: every instruction is fetched once per launch, at about 0.7 us a kilobyte, and four waves with four times the
+// code each took 14 to 18 us a launch
+template <int EPI>
+__global__ __launch_bounds__(1024) void ns_small_step(NsSmall p, NsGemm fin) {
+  __shared__ __attribute__((aligned(16))) f16x8_t af[2 * 32 * 64];   // A's fragments, then P's: chunk kk * 8 + mt
+  __shared__ __attribute__((aligned(16))) f16x8_t xf[2 * 16 * 64];   // the slice of X: chunk nt * 4 + kk
+  __shared__ __attribute__((aligned(16))) f16x8_t gf[SM_SLICE * SM_TLD / 4];   // its new rows for A, or the result in fp32
+  static_assert(SM_SLICE * SM_TLD / 4 >= 2 * 16 * 64, "both fit");
+  const int t = threadIdx.x, lane = t & 63, i15 = lane & 15, g = lane >> 4, z = blockIdx.y;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6), rw = w & 3, cw = w >> 2;
+  const int chunks = (int)(p.px >> 9);
+  f16x8_t* x = (f16x8_t*)(p.X + (long)z * 2 * p.px);
+  SmFrag xr = sm_get(x, chunks, blockIdx.x * 16 + w, lane);      // a sixteenth of the slice on its way to LDS
+  f32x4_t a[2][2], c[2][2], d[2][2];
+  sm_clear(a);
+  const f32x4_t* q = (const f32x4_t*)(p.gin + (long)z * p.parts * SM_PART) + (2 * rw * 8 + 2 * cw) * 64 + lane;
+  for (int k = 0; k < p.parts; k += 4) {                         // four parts on their way at a time
+    f32x4_t v[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j][i] = q[(long)min(k + j, p.parts - 1) * (SM_PART / 4) + ((i >> 1) * 8 + (i & 1)) * 64];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k + j < p.parts)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i >> 1][i & 1] += v[j][i];
+  }
+  const int kks = (p.m + 31) >> 5;                               // what lies behind row m is zero
+  constexpr float SC = 1.f / (float)(1L << (2 * SX - SA));
+  // one A for both terms of P: b A + c A^2 changes by (b + 2 c) of A's rounding near A = I, by 2 c if the terms' A differ
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const SmFrag f = sm_frag(a[i][0], a[i][1], SC);
+    sm_put(af, 32, cw * 8 + 2 * rw + i, lane, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[i][e >> 2][e & 3] = (float)f.h[e] + (float)f.l[e];
+  }
+  sm_clear(c);
+  sm_clear(d);
+  __syncthreads();
+#pragma unroll 1
+  for (int kk = 0; kk < kks; ++kk) {
+    const SmFrag f[2] = {sm_get(af, 32, kk * 8 + 2 * rw, lane), sm_get(af, 32, kk * 8 + 2 * rw + 1, lane)};
+    const SmFrag b[2] = {sm_get(af, 32, kk * 8 + 2 * cw, lane), sm_get(af, 32, kk * 8 + 2 * cw + 1, lane)};
+    sm_each([&](auto s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sm_mma<s.value>(c[i >> 1][i & 1], d[i >> 1][i & 1], b[i & 1], f[i >> 1]);
+    });
+  }
+  __syncthreads();                                               // A is read: each wave puts its part of P in its place
+  constexpr float PC = NS_C / (float)(1L << (2 * SA - SP)), PB = NS_B / (float)(1L << (SA - SP)), PA = NS_A * (float)(1L << SP);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        c[i][j][r] = (c[i][j][r] + d[i][j][r]) * PC + PB * a[i][j][r] + (2 * rw + i == 2 * cw + j && 4 * g + r == i15 ? PA : 0.f);
+    sm_put(af, 32, cw * 8 + 2 * rw + i, lane, sm_frag(c[i][0], c[i][1], 1.f));
+  }
+  constexpr float XC = 1.f / (float)(1L << SP);
+  sm_clear(c);
+  sm_clear(d);
+  for (int sl = blockIdx.x; sl < p.slices; sl += gridDim.x) {
+    sm_put(xf, 16, w, lane, xr);
+    if (sl + gridDim.x < p.slices) xr = sm_get(x, chunks, (sl + gridDim.x) * 16 + w, lane);
+    __syncthreads();
+    // 32 rows by 16 columns of P X: u with row 4 g + r and column i per lane (X's operand order), y with row i and column
+    // 4 g + r (the Gram matrix's); [small products][16 rows]
+    f32x4_t u[2][2], y[2][2];
+    sm_clear(u);
+    sm_clear(y);
+#pragma unroll 1
+    for (int kk = 0; kk < kks; ++kk) {
+      const SmFrag f[2] = {sm_get(af, 32, kk * 8 + 2 * rw, lane), sm_get(af, 32, kk * 8 + 2 * rw + 1, lane)};
+      const SmFrag b = sm_get(xf, 16, cw * 4 + kk, lane);
+      sm_each([&](auto s) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          sm_mma<s.value>(u[0][i], u[1][i], f[i], b);
+          if constexpr (EPI == NS_PLANES) sm_mma<s.value>(y[0][i], y[1][i], b, f[i]);
+        }
+      });
+    }
+    if constexpr (EPI == NS_PLANES) {
+      sm_put(x, chunks, sl * 16 + cw * 4 + rw, lane, sm_frag(u[0][0] + u[1][0], u[0][1] + u[1][1], XC));
+      const SmFrag f = sm_frag(y[0][0] + y[1][0], y[0][1] + y[1][1], XC);   // columns 16 cw ..: half of chunk cw / 2
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f16x4_t* o = (f16x4_t*)(gf + ((cw >> 1) * 8 + 2 * rw + i) * 64 + lane) + (cw & 1);
+        *o = f16x4_t{f.h[4 * i], f.h[4 * i + 1], f.h[4 * i + 2], f.h[4 * i + 3]};
+        o[16 * 64 * 2] = f16x4_t{f.l[4 * i], f.l[4 * i + 1], f.l[4 * i + 2], f.l[4 * i + 3]};
+      }
+      __syncthreads();
+      sm_gram(gf, rw, cw, lane, c, d);
+    } else {
+      float* tile = (float*)gf;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *(f32x4_t*)(tile + (16 * cw + i15) * SM_TLD + 32 * rw + 16 * i + 4 * g) = u[0][i] + u[1][i];
+      __syncthreads();
+      const int n = p.tall ? t >> 4 : 8 * (t & 7), m = p.tall ? 8 * (t & 15) : t >> 3;   // 8 columns of one row of the result
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p.tall ? tile[n * SM_TLD + m + e] : tile[(n + e) * SM_TLD + m];
+      const int n0 = sl * SM_SLICE;
+      ns_result8<EPI>(fin, z, p.tall ? n0 + n : m, p.tall ? m : n0 + n, v);
+    }
+    __syncthreads();
+  }
+  if constexpr (EPI == NS_PLANES) sm_part_out(p, rw, cw, lane, c, d);
+}
+
+struct SmSpace {
+  int slices, blocks;
+  long px;
+  double* part;
+  f16* X;
+  float *g[2], *sum;
+  size_t bytes;
+};
+static SmSpace sm_space(char* base, int B, int R, int C) {
+  SmSpace w;
+  w.slices = (max(R, C) + SM_SLICE - 1) / SM_SLICE;
+  w.blocks = min(w.slices, SM_BLOCKS);
+  w.px = (long)w.slices * SM_SLICE * NS_SMALL;
+  size_t o = 0;
+  auto take = [&](size_t n) {
+    char* p = base + o;
+    o += (n + 255) / 256 * 256;
+    return p;
+  };
+  w.part = (double*)take((size_t)B * NS_PARTS * 8);
+  w.X = (f16*)take((size_t)B * w.px * 4);
+  for (int i = 0; i < 2; ++i) w.g[i] = (float*)take((size_t)B * w.blocks * SM_PART * 4);
+  w.sum = (float*)take((size_t)B * SM_PART * 4);
+  w.bytes = o;
+  return w;
+}
+
+template <int KIND, int LAST>
+static int ns_small_run(const MuonIn& in, NsGemm fin, int B, int steps, float eps, char* ws, hipStream_t s) {
+  const SmSpace w = sm_space(ws, B, in.R, in.C);
+  NsSmall p{in, w.part, eps, w.X, w.px, nullptr, 0, w.g[0], min(in.R, in.C), max(in.R, in.C), w.slices, in.R > in.C};
+  const dim3 grid(w.blocks, B);
+  hipLaunchKernelGGL((muon_sumsq_kernel<KIND>), dim3(NS_PARTS, B), dim3(1024), 0, s, in, w.part);
+  NS_TRY(hipGetLastError());
+  hipLaunchKernelGGL((ns_small_first<KIND>), grid, dim3(1024), 0, s, p);
+  NS_TRY(hipGetLastError());
+  fin.R = in.R; fin.Cc = in.C; fin.il = in.il; fin.nb = in.B;
+  fin.cs = 1.f / (float)(1L << (SP + SX));
+  ns_set_vec(fin);
+  for (int k = 0; k < steps; ++k) {
+    p.gin = w.g[k & 1];
+    p.gout = w.g[~k & 1];
+    p.parts = w.blocks;
+    if (w.blocks > SM_DIRECT) {
+      hipLaunchKernelGGL(ns_small_sum, dim3(64, B), dim3(256), 0, s, p.gin, p.parts, w.sum);
+      NS_TRY(hipGetLastError());
+      p.gin = w.sum;
+      p.parts = 1;
+    }
+    if (k + 1 < steps) hipLaunchKernelGGL((ns_small_step<NS_PLANES>), grid, dim3(1024), 0, s, p, fin);
+    else hipLaunchKernelGGL((ns_small_step<LAST>), grid, dim3(1024), 0, s, p, fin);
+    NS_TRY(hipGetLastError());
+  }
+  return 0;
+}
+
 // the whole iteration; `fin` carries the last product's outputs
 template <int KIND, int LAST>
 static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float eps, char* ws, hipStream_t s) {
+  if (min(in.R, in.C) <= NS_SMALL) return ns_small_run<KIND, LAST>(in, fin, B, steps, eps, ws, s);
   const bool tall = in.R > in.C;
   // near-square matrices: single steps cost no more (7.5 n / m + 2.5 against 3 n / m + 7 products) and are more exact
   if (5L * max(in.R, in.C) <= 7L * min(in.R, in.C)) seg = 1;
@@ -813,8 +1139,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
       ap.B = b; ap.ldb = mp; ap.pb = tall ? w.ps : w.px; ap.bb = 2 * ap.pb;
       ap.M = Rp; ap.N = Cp; ap.K = mp; ap.cs = e2(-sq - SX);
       ap.R = in.R; ap.Cc = in.C; ap.il = in.il; ap.nb = in.B;
-      ap.vec = in.C % 8 == 0 && (uintptr_t)ap.C % 16 == 0 && (uintptr_t)ap.w % 16 == 0 && (uintptr_t)ap.copy % 16 == 0 &&
-               (uintptr_t)ap.lo % 16 == 0;
+      ns_set_vec(ap);
       NS_TRY(ns_launch<LAST>(ap, B, s));
     }
   }
@@ -831,6 +1156,7 @@ extern "C" {
 long dllm_muon_workspace(int B, int R, int C, int steps) {
   if (B <= 0 || B > 65535 || R <= 0 || C <= 0 || steps < 1 || steps > 20) return 0;
   if (pad128(min(R, C)) > 65536 || pad128(max(R, C)) > (1L << 21)) return 0;
+  if (min(R, C) <= NS_SMALL) return (long)sm_space(nullptr, B, R, C).bytes;
   return (long)ns_space(nullptr, B, R, C, steps > 1).bytes;
 }
 
