@@ -74,26 +74,33 @@ def fp8_empty(rows: int, k: int, fmt: str = "e4m3", device=None) -> BlockFP8:
 
 
 def _ld(t: torch.Tensor) -> int:
-    """Row stride of a row-major view (torch leaves the stride of a single row arbitrary)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    """Row stride of a view that ``_check_rows`` passed (torch leaves the stride of a single row arbitrary)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _check(q: BlockFP8, name: str) -> None:
+def _check(q: BlockFP8, name: str) -> tuple[int, int, int, int, int]:
+    """The operand as the kernels take it: (data, its row stride, scale, its row stride, format code)."""
     d, sc, k = q
-    if d.dtype not in _CODES or d.dim() != 2:
+    code = _CODES.get(d.dtype)
+    if code is None or d.dim() != 2:
         raise TypeError(f"{name}: data must be a 2-D float8 tensor (e4m3fn or e5m2), got {d.dtype} {tuple(d.shape)}")
     rows, cols = d.shape
-    if k < 0 or cols != -(-k // BLOCK) * BLOCK:
-        raise ValueError(f"{name}: data of k = {k} has {_blocks(k) * BLOCK} columns, got {cols}")
-    if sc.dtype != torch.uint8 or sc.shape != (cols // BLOCK, rows):
-        raise ValueError(f"{name}: scale must be uint8 {(_blocks(k), rows)}, got {sc.dtype} {tuple(sc.shape)}")
+    kb = -(-k // BLOCK)
+    if k < 0 or cols != kb * BLOCK:
+        raise ValueError(f"{name}: data of k = {k} has {kb * BLOCK} columns, got {cols}")
+    if sc.dtype != torch.uint8 or sc.shape != (kb, rows):
+        raise ValueError(f"{name}: scale must be uint8 {(kb, rows)}, got {sc.dtype} {tuple(sc.shape)}")
     if sc.device != d.device:
         raise ValueError(f"{name}: data on {d.device}, scale on {sc.device}")
+    ptr, (ld, s1), (lds, t1) = d.data_ptr(), d.stride(), sc.stride()
+    ld, lds = ld if rows > 1 else cols, lds if kb > 1 else rows
     if rows and cols:
-        if d.stride(1) != 1 or (rows > 1 and sc.stride(1) != 1):
-            raise ValueError(f"{name}: data and scale must be contiguous along their last dimension")
-        if d.is_cuda and (d.data_ptr() % 16 or _ld(d) % 16):
+        if s1 != 1 or (rows > 1 and t1 != 1) or ld < cols or lds < rows:
+            raise ValueError(f"{name}: data and scale must be contiguous along their last dimension, without overlapping rows; "
+                             f"got strides {d.stride()} and {sc.stride()}")
+        if d.is_cuda and (ptr % 16 or ld % 16):
             raise ValueError(f"{name}: data rows must start at multiples of 16 bytes")
+    return ptr, ld, sc.data_ptr(), lds, code
 
 
 def _pow2(e: torch.Tensor) -> torch.Tensor:
@@ -118,25 +125,28 @@ def _quantize_torch(x: torch.Tensor, dt: torch.dtype, tile: bool, out: BlockFP8)
     out.scale.copy_((e + 127).to(torch.uint8).expand(v.shape[0], v.shape[1], kb, 1).reshape(-1, kb)[:R].t())
 
 
-def _check_out(o: BlockFP8, rows: int, k: int, device, name: str) -> BlockFP8:
-    _check(o, name)
-    if o.rows != rows or o.k != k or o.device != device:
-        raise ValueError(f"{name} must hold {(rows, k)} on {device}, got {(o.rows, o.k)} on {o.device}")
-    return o
+def _target(out: BlockFP8 | None, rows: int, k: int, fmt: str, device, name: str) -> tuple[BlockFP8, tuple]:
+    """The output operand (made, or checked) and the kernels' form of it."""
+    if out is None:
+        out = fp8_empty(rows, k, fmt, device)
+        return out, (out.data.data_ptr(), out.data.shape[1], out.scale.data_ptr(), rows, _CODES[out.data.dtype])
+    arg = _check(out, name)
+    if out.rows != rows or out.k != k or out.device != device:
+        raise ValueError(f"{name} must hold {(rows, k)} on {device}, got {(out.rows, out.k)} on {out.device}")
+    return out, arg
 
 
 def _shape2(x: torch.Tensor) -> tuple[int, int]:
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+    if x.dim() != 2 or x.dtype not in _native.DT:
         raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
     return x.shape
 
 
-def _arg(o: BlockFP8 | None) -> tuple:
-    return (None, 0, None, 0) if o is None else (o.data.data_ptr(), _ld(o.data), o.scale.data_ptr(), _ld(o.scale))
+_NONE = (None, 0, None, 0, 0)
 
 
-def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bool) -> None:
-    R, C = x.shape
+def _quantize(x: torch.Tensor, R: int, C: int, q: BlockFP8 | None, arg: tuple, qt: BlockFP8 | None, arg_t: tuple,
+              tile: bool) -> None:
     if R == 0 or C == 0:
         return
     if not x.is_cuda:
@@ -147,11 +157,10 @@ def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bo
         return
     if C > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    with _on(x.device):
-        rc = _native.lib().dllm_fp8_quantize(x.data_ptr(), _native.DT[x.dtype], x.stride(0), R, C, *_arg(q), *_arg(qt),
-                                             _CODES[q.data.dtype] if q is not None else 0,
-                                             _CODES[qt.data.dtype] if qt is not None else 0, int(tile),
-                                             _native.stream_ptr(x.device))
+    dev = x.device
+    with _on(dev):
+        rc = _native.lib().dllm_fp8_quantize(x.data_ptr(), _native.DT[x.dtype], x.stride(0), R, C, *arg[:4], *arg_t[:4], arg[4],
+                                             arg_t[4], int(tile), _native.stream_ptr(dev))
     if rc:
         _native.check(rc, f"dllm_fp8_quantize({R}x{C})")
 
@@ -159,16 +168,16 @@ def _quantize(x: torch.Tensor, q: BlockFP8 | None, qt: BlockFP8 | None, tile: bo
 def quantize_fp8(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
     """The 8-bit form of ``x`` [R, K] (bf16 / fp32), scaled per row and 128 columns (``tile``: per 128x128 tile)."""
     R, C = _shape2(x)
-    out = fp8_empty(R, C, fmt, x.device) if out is None else _check_out(out, R, C, x.device, "out")
-    _quantize(x, out, None, tile)
+    out, arg = _target(out, R, C, fmt, x.device, "out")
+    _quantize(x, R, C, out, arg, None, _NONE, tile)
     return out
 
 
 def quantize_fp8_t(x: torch.Tensor, fmt: str = "e4m3", *, tile: bool = False, out: BlockFP8 | None = None) -> BlockFP8:
     """The 8-bit form of ``xᵀ`` [K, R], scaled per column of ``x`` and 128 rows (``tile``: per 128x128 tile)."""
     R, C = _shape2(x)
-    out = fp8_empty(C, R, fmt, x.device) if out is None else _check_out(out, C, R, x.device, "out")
-    _quantize(x, None, out, tile)
+    out, arg = _target(out, C, R, fmt, x.device, "out")
+    _quantize(x, R, C, None, _NONE, out, arg, tile)
     return out
 
 
@@ -177,22 +186,26 @@ def quantize_fp8_both(x: torch.Tensor, fmt: str = "e4m3", fmt_t: str = "e4m3", *
     """``(quantize_fp8(x, fmt), quantize_fp8_t(x, fmt_t))`` from one read of ``x``: a forward (or input-gradient) operand
     and the weight-gradient operand of the same tensor."""
     R, C = _shape2(x)
-    out = fp8_empty(R, C, fmt, x.device) if out is None else _check_out(out, R, C, x.device, "out")
-    out_t = fp8_empty(C, R, fmt_t, x.device) if out_t is None else _check_out(out_t, C, R, x.device, "out_t")
-    _quantize(x, out, out_t, tile)
+    out, arg = _target(out, R, C, fmt, x.device, "out")
+    out_t, arg_t = _target(out_t, C, R, fmt_t, x.device, "out_t")
+    _quantize(x, R, C, out, arg, out_t, arg_t, tile)
     return out, out_t
 
 
 def dequantize_fp8(q: BlockFP8, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """The values ``[rows, k]`` that ``q`` stands for, in bf16 or fp32: exact but where the type ends (a code that rounded up
     to 2^128 reads as inf; values among the type's subnormals are rounded)."""
-    _check(q, "q")
-    d, sc, k = q
+    ptr, ld, sptr, lds, code = _check(q, "q")
+    d, k = q.data, q.k
     rows, dev = d.shape[0], d.device
+    dtype = dtype if out is None else out.dtype
+    if dtype not in _native.DT:
+        raise TypeError(f"dequantize_fp8 gives bf16 or fp32, not {dtype}")
     if out is None:
-        out = torch.empty((rows, k), dtype=dtype, device=dev)
-    if out.shape != (rows, k) or out.device != dev or out.dtype not in _native.DT:
-        raise ValueError(f"out must be bf16 or fp32 {(rows, k)} on {dev}")
+        out, ldo = torch.empty((rows, k), dtype=dtype, device=dev), k
+    else:
+        _check_rows(out, "out", (rows, k), dev)
+        ldo = _ld(out)
     if rows == 0 or k == 0:
         return out
     if not d.is_cuda:
@@ -203,10 +216,9 @@ def dequantize_fp8(q: BlockFP8, dtype: torch.dtype = torch.float32, out: torch.T
         v = torch.where((e == 128).unsqueeze(2), torch.full_like(v, float("nan")), v)
         out.copy_(v.reshape(q.rows, -1)[:, :q.k])
         return out
-    _check_rows(out, "out", (rows, k), dev)
     with _on(dev):
-        rc = _native.lib().dllm_fp8_dequantize(d.data_ptr(), _ld(d), sc.data_ptr(), _ld(sc), _CODES[d.dtype], out.data_ptr(),
-                                               _native.DT[out.dtype], _ld(out), rows, k, _native.stream_ptr(dev))
+        rc = _native.lib().dllm_fp8_dequantize(ptr, ld, sptr, lds, code, out.data_ptr(), _native.DT[dtype], ldo, rows, k,
+                                               _native.stream_ptr(dev))
     if rc:
         _native.check(rc, f"dllm_fp8_dequantize({rows}x{k})")
     return out
@@ -241,24 +253,24 @@ def gemm_fp8(a: BlockFP8, b: BlockFP8, out: torch.Tensor | None = None, *, out_d
     The result's type sets the arithmetic.  fp32: exact products and fp32 sums (about 5e-7 of the result at K = 8192), at
     the bf16 matrix rate.  bf16: the 8-bit matrix instruction, twice as fast, whose sums of 8 neighbouring products keep 13
     bits below the largest (about 4e-5 of the result, a hundredth of bf16's half step)."""
-    _check(a, "a")
-    _check(b, "b")
-    ad, asc, k = a
-    bd, bsc, kb = b
+    aarg, barg = _check(a, "a"), _check(b, "b")
+    ad, bd, k = a.data, b.data, a.k
     dev = ad.device
-    if k != kb:
-        raise ValueError(f"gemm_fp8: inner dims differ ({k} vs {kb})")
+    if k != b.k:
+        raise ValueError(f"gemm_fp8: inner dims differ ({k} vs {b.k})")
     if dev != bd.device:
         raise ValueError(f"gemm_fp8: operands on {dev} and {bd.device}")
     M, N = ad.shape[0], bd.shape[0]
     if out is None:
         if beta != 0.0:
             raise ValueError("gemm_fp8: beta needs out")
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=dev), N
     else:
         _check_rows(out, "out", (M, N), dev)
-    if out.dtype not in _native.DT:
-        raise TypeError(f"gemm_fp8: out must be bf16 or fp32, got {out.dtype}")
+        ldc, out_dtype = _ld(out), out.dtype
+    oc = _native.DT.get(out_dtype)
+    if oc is None:
+        raise TypeError(f"gemm_fp8: out must be bf16 or fp32, got {out_dtype}")
     side = None
     if epi == "store":
         if aux is not None or aux_out is not None:
@@ -271,13 +283,12 @@ def gemm_fp8(a: BlockFP8, b: BlockFP8, out: torch.Tensor | None = None, *, out_d
         return out
     if not ad.is_cuda:
         return _gemm_torch(a, b, out, alpha, beta, epi, act, aux, aux_out)
-    oc, nk = _native.DT[out.dtype], _blocks(k)
+    nk = ad.shape[1] // BLOCK
     tile, ksplit = _plan(M, N, nk, oc)
     ws = torch.empty(ksplit * M * N, dtype=torch.float32, device=dev) if ksplit > 1 else None
     with _on(dev):
         rc = _native.lib().dllm_fp8_gemm(
-            ad.data_ptr(), _ld(ad), asc.data_ptr(), _ld(asc), _CODES[ad.dtype], bd.data_ptr(), _ld(bd), bsc.data_ptr(),
-            _ld(bsc), _CODES[bd.dtype], out.data_ptr(), _ld(out), oc, aux.data_ptr() if aux is not None else None,
+            *aarg, *barg, out.data_ptr(), ldc, oc, aux.data_ptr() if aux is not None else None,
             aux_out.data_ptr() if aux_out is not None else None, _ld(side) if side is not None else 0, M, N, nk, alpha, beta,
             EPIS[epi], code, tile, ksplit, ws.data_ptr() if ws is not None else None, _native.stream_ptr(dev))
     if rc:

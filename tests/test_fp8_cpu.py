@@ -176,6 +176,10 @@ def test_refusals():
         fp8.dequantize_fp8(q._replace(scale=q.scale[:, :3]))
     with pytest.raises(ValueError, match="contiguous along"):
         fp8.dequantize_fp8(q._replace(scale=q.scale.t().contiguous().t()))
+    for bad in (q._replace(data=q.data[:1].expand(q.rows, -1)), q._replace(scale=q.scale[:1].expand(len(q.scale), -1))):
+        if bad.data.stride(0) == 0 or len(bad.scale) > 1:          # one row standing for all: the kernels step over rows
+            with pytest.raises(ValueError, match="overlapping rows"):
+                fp8.dequantize_fp8(bad)
     with pytest.raises(ValueError, match="out must be"):
         fp8.dequantize_fp8(q, out=torch.empty(4, 100))
     with pytest.raises(ValueError, match="inner dims"):
