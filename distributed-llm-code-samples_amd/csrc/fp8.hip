@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* q, l
 // chunks g and 4 + g (g = lane / 16) of its row, in A and B alike: a permutation of k inside the block, which neither the
 // sum nor the block's one scale sees.  The operands are swapped in the matrix instruction (B first), so a lane ends with
 // consecutive columns of a row of C.  Three kernels: 256x256 tiles (8-phase loop), 128x128 and 64x64 tiles (one wave per
-// quarter), and few rows or columns (operands straight to registers, K over the waves); dllm_fp8_gemm picks.
+// quarter), and few rows or columns (operands straight to registers, K over the waves); fp8_plan picks.
 // ----------------------------------------------------------------------------------------------
 template <int FB, int FA>
 __device__ __forceinline__ f32x4_t mfma_f8(i32x8_t b, i32x8_t a, f32x4_t c, int sb, int sa) {
@@ -684,16 +684,19 @@ __global__ __launch_bounds__(256) void fp8_join(Fp8GemmArgs p) {
 // ----------------------------------------------------------------------------------------------
 // few rows of A (SWAP: of B), at most 16 MT: 16 rows of the other operand per block, the K steps dealt to its 8 waves
 //
-// Bound by reading the long operand once (and by latency: everything a wave needs for 4 steps is requested at once).
 // Fragments go from memory to registers (a step's line of a row is read by the 4 lanes of its row), the waves' sums are
-// added in LDS in the order of the waves.
+// added in LDS in the order of the waves.  At one row bound by reading the long operand (16384 x 4096 in 14.7 us, 4.6 TB/s);
+// with more rows by reading the short operand again for every 16 rows of the long one, from L2: 16 rows 19.7 us, 64 rows 46.
+// 64x64 tiles read it once per 64 (19.0 us), so fp8_plan takes them there; on a small long operand they leave CUs empty
+// (1024 x 1024, 64 rows: 5.4 us here, 6.4 there).
 // ----------------------------------------------------------------------------------------------
 template <int EPI, typename OutT, int FA, int FB, int MT, bool SWAP>
 __global__ __launch_bounds__(512) void fp8_gemm_rows(Fp8GemmArgs p) {
   __shared__ f32x4_t part[8][MT][64];
   constexpr bool EXACT = sizeof(OutT) == 4;
   constexpr int FS = SWAP ? FB : FA, FL = SWAP ? FA : FB;        // formats of the short and the long operand
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6, i15 = lane & 15, g = lane >> 4;
+  const int t = threadIdx.x, lane = t & 63, i15 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint8_t *L = SWAP ? p.A : p.B, *SL = SWAP ? p.SA : p.SB, *S = SWAP ? p.B : p.A, *SS = SWAP ? p.SB : p.SA;
   const long ldl = SWAP ? p.lda : p.ldb, ldsl = SWAP ? p.ldsa : p.ldsb, lds = SWAP ? p.ldb : p.lda, ldss = SWAP ? p.ldsb : p.ldsa;
   const int nl = SWAP ? p.M : p.N, ns = SWAP ? p.N : p.M;
@@ -713,23 +716,45 @@ __global__ __launch_bounds__(512) void fp8_gemm_rows(Fp8GemmArgs p) {
     const n8_i32x4 lo = *(const n8_i32x4*)q, hi = *(const n8_i32x4*)(q + 64);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  constexpr int U = MT == 4 ? 2 : 4;
-#pragma unroll U
-  for (int kt = w; kt < p.nk; kt += 8) {
-    const i32x8_t fl = load(lp + (long)kt * 128);
-    const int sl = SL[(long)kt * ldsl + rl];
+  // the loads of D steps are on their way together: one step at a time waits for memory at each (32 rows by 4096 x 4096:
+  // 10.5 us, now 8.7)
+  constexpr int D = MT == 4 ? 2 : 4;
+  for (int kt = w; kt < p.nk; kt += 8 * D) {
+    i32x8_t fl[D], fs[D][MT];
+    int sl[D], ss[D][MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const i32x8_t fs = load(sp[i] + (long)kt * 128);
-      const int ss = SS[(long)kt * ldss + rs[i]];
-      if constexpr (!EXACT) {
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fl, fs, acc[i], FL, FS, 0, sl, 0, ss);
-      } else {
-        const float a = __uint_as_float((uint32_t)ss << 23), b = __uint_as_float((uint32_t)sl << 23);
+    for (int d = 0; d < D; ++d) {
+      if (kt + 8 * d >= p.nk) break;
+      const int k = kt + 8 * d;
+      fl[d] = load(lp + (long)k * 128);
+      sl[d] = SL[(long)k * ldsl + rl];
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<FL>(fl[2 * s], fl[2 * s + 1], b),
-                                                           codes8<FS>(fs[2 * s], fs[2 * s + 1], a), acc[i], 0, 0, 0);
+      for (int i = 0; i < MT; ++i) {
+        fs[d][i] = load(sp[i] + (long)k * 128);
+        ss[d][i] = SS[(long)k * ldss + rs[i]];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {   // uses that stay here: the compiler moves loads down to their first use
+      asm volatile("" : "+v"(fl[d]), "+v"(sl[d]));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) asm volatile("" : "+v"(fs[d][i]), "+v"(ss[d][i]));
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (kt + 8 * d >= p.nk) break;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (!EXACT) {
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fl[d], fs[d][i], acc[i], FL, FS, 0, sl[d], 0, ss[d][i]);
+        } else {
+          const float a = __uint_as_float((uint32_t)ss[d][i] << 23), b = __uint_as_float((uint32_t)sl[d] << 23);
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(codes8<FL>(fl[d][2 * s], fl[d][2 * s + 1], b),
+                                                             codes8<FS>(fs[d][i][2 * s], fs[d][i][2 * s + 1], a), acc[i], 0, 0, 0);
+        }
       }
     }
   }
@@ -764,7 +789,7 @@ static int fp8_cus() {
 template <int EPI, typename OutT, int FA, int FB>
 static hipError_t launch_fp8_f(Fp8GemmArgs p, hipStream_t s) {
   const int few = min(p.M, p.N);
-  if (few <= 64) {
+  if (p.tile == 0) {
     const bool swap = p.N < p.M;
     const dim3 grid((unsigned)((max(p.M, p.N) + 15) / 16)), block(512);
     auto go = [&](auto mt, auto sw) {
@@ -804,14 +829,26 @@ static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s
   return fb == F8_E4M3 ? launch_fp8_f<EPI, OutT, F8_E5M2, F8_E4M3>(p, s) : launch_fp8_f<EPI, OutT, F8_E5M2, F8_E5M2>(p, s);
 }
 
-// Tile and number of K slices: the least time for whole rounds of CUs, in microseconds measured on full rounds: a K step of
-// 128 on one CU (bf16 results / fp32 results), a round's beginning and end, and the slices' partial sums at 1.5 TB/s.
+constexpr int FP8_FEW = 64;   // rows (or columns) that fp8_gemm_rows takes, at most
+
+// Tile (0: fp8_gemm_rows) and number of K slices: the least time for whole rounds of CUs, in microseconds measured on full
+// rounds: a K step of 128 on one CU (bf16 results / fp32 results), a round's beginning and end, and the slices' partial sums
+// at 1.5 TB/s.  Every choice was measured at six weights (1024 x 1024 to 16384 x 4096) and nine numbers of rows (1 to 256):
+// the one it makes is the fastest or within 13 % of it, and once 23 % (2048 x 8192, 256 rows: 24.8 us, two slices 20.2).
 static void fp8_plan(int M, int N, int nk, bool exact, int& tile, int& ksplit) {
   struct { int ts, blocks; float fast, exact; } kinds[] = {{256, 1, 1.45f, 3.0f}, {128, 1, 0.42f, 0.75f}, {64, 2, 0.30f, 0.40f}};
   float best = 1e30f;
   tile = 128;
   ksplit = 1;
   const long cus = fp8_cus();
+  const int few = (min(M, N) + 15) / 16 * 16;
+  if (few <= FP8_FEW) {
+    // a block reads its 16 long rows and all of the short operand, at about 30 KB/us on a CU
+    const long blocks = (max(M, N) + 15) / 16;
+    best = (float)((blocks + cus - 1) / cus) * (float)(few + 16) * (float)nk * (128.f / 30e3f) + 3.f;
+    tile = 0;
+    if (few == 16) return;
+  }
   for (auto& k : kinds) {
     const long tiles = (long)((M + k.ts - 1) / k.ts) * ((N + k.ts - 1) / k.ts);
     for (int s = 1; s <= 8; s *= 2) {
@@ -894,9 +931,11 @@ int dllm_fp8_gemm(const void* A, long lda, const void* SA, long ldsa, int fa, co
   if ((aux || aux_out) && ldaux < N) return -1;
   Fp8GemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)SA, ldsa, (const uint8_t*)B, ldb, (const uint8_t*)SB, ldsb,
                 C, ldc, aux, aux_out, ldaux, M, N, nk, alpha, beta, act, tile, ksplit, ws};
-  if (min(M, N) > 64) {
+  if (tile == 0) {
+    if (min(M, N) > FP8_FEW || ksplit != 1) return -1;
+  } else {
     // the buffer-form fetches reach 2^31 bytes from a tile's first row; scale words span 4 (2) rows, which these have
-    if ((tile != 64 && tile != 128 && tile != 256) || ksplit < 1 || ksplit > 8 || (ksplit > 1 && (ws == nullptr || tile == 256)))
+    if (min(M, N) <= 16 || (tile != 64 && tile != 128 && tile != 256) || ksplit < 1 || ksplit > 8 || (ksplit > 1 && (ws == nullptr || tile == 256)))
       return -1;
     if (max(lda, ldb) > (0x7fffffffL - 4096) / 256 || (nk == 0 && tile == 256)) return -1;
   }

@@ -231,14 +231,9 @@ def _check_rows(t: torch.Tensor, name: str, shape: tuple, device) -> None:
         raise ValueError(f"{name} must be a row-major view without overlapping rows, got strides {t.stride()}")
 
 
-_FEW = 64   # products with at most this many rows or columns take no tile plan (csrc/fp8.hip fp8_gemm_rows)
-
-
 @functools.lru_cache(maxsize=4096)
 def _plan(M: int, N: int, kb: int, out_code: int) -> tuple[int, int]:
-    """(output tile, K slices) of a product's sizes and result type."""
-    if min(M, N) <= _FEW:
-        return 0, 1
+    """(output tile, or 0 for the kernel for few rows, K slices) of a product's sizes and result type."""
     p = _native.lib().dllm_fp8_gemm_plan(M, N, kb, out_code)
     return p & 0xFFFF, p >> 16
 

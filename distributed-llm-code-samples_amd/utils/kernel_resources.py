@@ -4,7 +4,7 @@ The 8-phase GEMM schedule assumes every production instantiation runs spill-free
 (scratch) segment puts scratch loads and stores -- and the ``s_waitcnt vmcnt(0)`` hipcc emits around them -- inside
 the counted-``vmcnt`` main loop, which both drains the LDS-DMA pipeline and, in round 5, preceded a GPU memory-
 aperture fault in a diagnostic build that spilled (docs/DESIGN.md §2).  ``check_built()`` extracts the gfx950 code
-object from each built GEMM object (``build/gemm*.hip.o``: offload bundle in ``.hip_fatbin``), parses the AMDGPU
+object from each built GEMM object (``build/gemm*``, ``fp8``, ``muon`` ``.hip.o``: offload bundle in ``.hip_fatbin``), parses the AMDGPU
 metadata notes and returns every budget violation; ``tests/test_kernel_resources_cpu.py`` runs it in the CPU suite.
 
     python -m dllm.utils.kernel_resources            # table of the GEMM kernels + violations
@@ -34,6 +34,18 @@ FAMILIES = (
     ("_ZN4dllm13gemm_bf16_256I", 256, None),
     ("_ZN4dllm12gemm_f32_256I", 256, None),
     ("_ZN4dllm12gemm_f32_128I", 256, None),
+    # block-scaled 8-bit and two-plane fp16 products: 256x256 on the 8-phase loop (8 half-tiles), 64x64 (4 K steps of 16 KiB)
+    # and 128x128 (dynamic LDS) at 256 registers; 192x192 has one wave per SIMD and the whole 512-entry file (3 K steps)
+    ("_ZN4dllm12fp8_gemm_256I", 256, (131072,)),
+    ("_ZN4dllm12fp8_gemm_128I", 256, (0,)),
+    ("_ZN4dllm11fp8_gemm_64I", 256, (65536,)),
+    ("_ZN4dllm11ns_gemm_256I", 256, (131072,)),
+    ("_ZN4dllm11ns_gemm_128I", 256, (0,)),
+    ("_ZN4dllm10ns_gemm_64I", 256, (65536,)),
+    ("_ZN4dllm11ns_gemm_192I", 512, (147456,)),
+    # 16 waves per block: 128 registers
+    ("_ZN4dllm13ns_small_stepI", 128, None),
+    ("_ZN4dllm14ns_small_firstI", 128, None),
 )
 LDS_MAX = 160 * 1024
 
@@ -83,10 +95,9 @@ def violations(recs: list[dict], families=FAMILIES) -> list[str]:
             bad.append(f"{r['name']}: {r['lds']} B of LDS > {LDS_MAX}")
         for prefix, regs, lds in families:
             if r["name"].startswith(prefix):
-                # the unified register file: arch VGPRs (allocated in granules of 8) + AGPRs per lane
-                used = -(-r["vgpr"] // 8) * 8 + r["agpr"]
-                if used > regs:
-                    bad.append(f"{r['name']}: {r['vgpr']} VGPR + {r['agpr']} AGPR > {regs}")
+                # the unified register file, in granules of 8 per lane: vgpr_count holds the AGPRs too
+                if -(-r["vgpr"] // 8) * 8 > regs:
+                    bad.append(f"{r['name']}: {r['vgpr']} VGPR ({r['agpr']} of them AGPR) > {regs}")
                 if lds is not None and r["lds"] not in lds:
                     bad.append(f"{r['name']}: {r['lds']} B of LDS, the schedule assumes one of {lds}")
     return bad
@@ -94,7 +105,7 @@ def violations(recs: list[dict], families=FAMILIES) -> list[str]:
 
 def built_objects(build_dir: str = BUILD) -> list[str]:
     return sorted(os.path.join(build_dir, f) for f in os.listdir(build_dir)
-                  if f.startswith("gemm") and f.endswith(".hip.o"))
+                  if f.startswith(("gemm", "fp8", "muon")) and f.endswith(".hip.o"))
 
 
 def check_built(build_dir: str = BUILD) -> tuple[list[dict], list[str]]:

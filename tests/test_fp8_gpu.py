@@ -107,7 +107,7 @@ def test_gemm(M, N, K, fa, fb, out):
     product_check(fp8.gemm_fp8(qa, qb, c, alpha=0.75, beta=-0.5), qa, qb, 0.75, -0.5, c0)
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 33000, 300), (2817, 3001, 513), (33000, 5, 128), (4096, 2048, 256), (4, 32768, 640),
+@pytest.mark.parametrize("M,N,K", [(5, 33000, 300), (40, 17000, 1000), (17000, 23, 1000), (50, 2049, 8200), (2817, 3001, 513), (33000, 5, 128), (4096, 2048, 256), (4, 32768, 640),
                                    (2900, 3100, 1100)])
 @pytest.mark.parametrize("fa,fb", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
