@@ -28,6 +28,7 @@ from .activations import act_code, act_fwd, act_grad
 from .gemm import EPIS
 
 BLOCK = 128
+MAX_DIM = 2 ** 31 - 2 * BLOCK      # the kernels count rows and columns in 32 bits
 FORMATS = {"e4m3": torch.float8_e4m3fn, "e5m2": torch.float8_e5m2}
 _CODES = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
 _TOP = {torch.float8_e4m3fn: 8, torch.float8_e5m2: 15}   # FMAX = 1.75 * 2^top
@@ -85,6 +86,8 @@ def _check(q: BlockFP8, name: str) -> tuple[int, int, int, int, int]:
     if code is None or d.dim() != 2:
         raise TypeError(f"{name}: data must be a 2-D float8 tensor (e4m3fn or e5m2), got {d.dtype} {tuple(d.shape)}")
     rows, cols = d.shape
+    if rows > MAX_DIM or cols > MAX_DIM:
+        raise ValueError(f"{name}: up to {MAX_DIM} rows and columns, got {rows} and {cols}")
     kb = -(-k // BLOCK)
     if k < 0 or cols != kb * BLOCK:
         raise ValueError(f"{name}: data of k = {k} has {kb * BLOCK} columns, got {cols}")
@@ -139,7 +142,10 @@ def _target(out: BlockFP8 | None, rows: int, k: int, fmt: str, device, name: str
 def _shape2(x: torch.Tensor) -> tuple[int, int]:
     if x.dim() != 2 or x.dtype not in _native.DT:
         raise TypeError(f"the quantiser takes 2-D bf16 or fp32 tensors, got {x.dtype} {tuple(x.shape)}")
-    return x.shape
+    R, C = x.shape
+    if R > MAX_DIM or C > MAX_DIM:
+        raise ValueError(f"the quantiser takes up to {MAX_DIM} rows and columns, got {tuple(x.shape)}")
+    return R, C
 
 
 _NONE = (None, 0, None, 0, 0)

@@ -47,7 +47,7 @@ def _check_dense(t: torch.Tensor, name: str, shape: torch.Size, dtypes: tuple, d
 
 
 def _workspace(B: int, R: int, C: int, steps: int, device) -> torch.Tensor:
-    n = _native.lib().dllm_muon_workspace(B, R, C, steps)
+    n = _native.lib().dllm_muon_workspace(B, R, C, steps) if max(B, R, C) < 2 ** 31 else 0
     if n <= 0:
         raise ValueError(f"matrices of {R}x{C} (batch {B}) are beyond the kernels' range: shorter side up to 65536, "
                          "longer up to 2097152, batch up to 65535")
@@ -106,6 +106,11 @@ def _blocks_of(t: torch.Tensor, interleave: int) -> torch.Tensor:
     return t.view(-1, 2, interleave, C).transpose(0, 1).reshape(2, -1, C)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
+
+
 def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, interleave, master, copy, lo) -> None:
     ref = lo if master is None else master
     B, R, C = _dims(ref, "the weight")
@@ -122,6 +127,13 @@ def _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale,
         B, R = 2, R // 2
     if ref.numel() == 0:
         return
+    # the momentum is written while the gradient is read, and both are read again when the weights are written
+    for t, what in ((grad, "grad"), (momentum, "momentum")):
+        for u in (momentum, ref, copy) if t is grad else (ref, copy):
+            if u is not None and _overlap(t, u):
+                raise ValueError(f"{what} must not share memory with the other tensors")
+    if copy is not None and _overlap(ref, copy):
+        raise ValueError("the weight's tensors must not share memory")
     rate = lr * (muon_scale(R, C) if scale is None else scale)
     decay = 1.0 - lr * wd
     if ref.device.type != "cuda":

@@ -166,6 +166,9 @@ def test_refusals():
         fp8.quantize_fp8(x.half())
     with pytest.raises(TypeError, match="2-D bf16 or fp32"):
         fp8.quantize_fp8(x[0])
+    for shape in ((2 ** 31, 1), (1, 2 ** 31)):
+        with pytest.raises(ValueError, match="rows and columns"):
+            fp8.quantize_fp8(torch.zeros(1, 1).expand(shape))
     with pytest.raises(ValueError, match="must hold"):
         fp8.quantize_fp8(x, out=fp8.fp8_empty(4, 100))
     with pytest.raises(TypeError, match="float8"):

@@ -202,6 +202,21 @@ def test_gemm_non_finite():
     assert torch.equal(torch.isfinite(y), torch.isfinite(want)) and torch.equal(torch.isnan(y), torch.isnan(want))
 
 
+@pytest.mark.parametrize("M,N", [(3, 70), (40, 90), (130, 300), (70, 5)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_gemm_scale_nan(M, N, out):
+    """Scale byte 255 stands for NaN: its block's row (column) of the result is NaN, the rest is untouched."""
+    qa, qb = fp8.quantize_fp8(rand(M, 300, 8).to(DEV)), fp8.quantize_fp8(rand(N, 300, 9).to(DEV), "e5m2")
+    clean = fp8.gemm_fp8(qa, qb, out_dtype=out)
+    qa.scale[1, 2] = 255
+    qb.scale[2, 4] = 255
+    y = fp8.gemm_fp8(qa, qb, out_dtype=out)
+    assert torch.isnan(y[2]).all() and torch.isnan(y[:, 4]).all() and torch.isnan(fp8.dequantize_fp8(qa)[2, 128:256]).all()
+    rest = torch.ones(M, N, dtype=torch.bool, device=DEV)
+    rest[2], rest[:, 4] = False, False
+    assert torch.equal(y[rest], clean[rest])
+
+
 def test_gemm_scale_extremes():
     """Scales from 2^-127 to 2^120: products far outside fp32 become 0 or inf as fp32 arithmetic would have them."""
     x = torch.cat([torch.full((20, 128), 1e-38), torch.full((20, 128), 1e30), torch.full((20, 128), 1.0),

@@ -95,5 +95,11 @@ def test_refusals():
         muon.muon_step_(x, x.clone(), torch.randn(6, 4).t(), lr=0.1)
     with pytest.raises(TypeError, match="copy must be"):
         muon.muon_step_(x, x.clone(), x.clone(), lr=0.1, copy=x.clone())
+    for w, g, m in ((x, x, x.clone()), (x, x.clone(), x)):
+        with pytest.raises(ValueError, match="share memory"):
+            muon.muon_step_(w, g, m, lr=0.1)
+    both = torch.randn(7, 4)
+    with pytest.raises(ValueError, match="share memory"):        # overlapping by all but a row
+        muon.muon_step_(torch.randn(6, 4), both[:6], both[1:], lr=0.1)
     with pytest.raises(TypeError, match="int16 residual"):
         muon.muon_split_step_(x, x.bfloat16(), x, x.clone(), lr=0.1)
