@@ -14,18 +14,30 @@ typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 // quantiser: one block of 256 threads per 128x128 tile of x, one read of x for both orientations
 //
 // Thread (g, j) = (t / 16, t % 16) holds rows 8g .. 8g+7 and columns 8j .. 8j+7 of the tile in registers.  A row's 128
-// columns sit in 16 neighbouring lanes (row scales: 4 lane exchanges), a column's 128 rows in 16 values of g (column
-// scales: lane exchanges over the wave's four g, then LDS over the four waves).  x^T leaves through LDS so that its rows
-// are written in whole 128-B lines.  Bound by HBM: reads x once and writes one byte per element and orientation.
+// columns sit in 16 neighbouring lanes (row scales: 4 rotations within them), a column's 128 rows in 16 values of g (column
+// scales: two lane exchanges that leave each of the wave's four g with two of the eight columns, then LDS over the four
+// waves).  x^T leaves through LDS so that its rows are written in whole 128-B lines; its rows there are 33 words apart, which
+// spreads both the writes and the reads over all banks.
 // ----------------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf2f(v); }
 template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
 
-// magnitude bits of v, 0 for inf / NaN (the block's scale comes from its finite elements)
+// magnitude bits of v (in the order of magnitudes, then inf, then NaN), and the same with 0 for inf / NaN: a block's scale
+// comes from its finite elements.  Integers: a float maximum gives way to a signalling NaN
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  const uint32_t b = abs_bits(v);
   return b < 0x7f800000u ? b : 0u;
+}
+
+// max over the 16 lanes of a row, in all of them
+__device__ __forceinline__ uint32_t max_row16(uint32_t m) {
+  auto ror = [](uint32_t x, auto n) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + n.value, 0xf, 0xf, false); };
+  m = max(m, ror(m, std::integral_constant<int, 8>{}));
+  m = max(m, ror(m, std::integral_constant<int, 4>{}));
+  m = max(m, ror(m, std::integral_constant<int, 2>{}));
+  return max(m, ror(m, std::integral_constant<int, 1>{}));
 }
 
 // four values (already scaled into range) -> four 8-bit codes.  Rounds to nearest even; |v| <= FMAX by construction, so
@@ -42,15 +54,22 @@ __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   }
   return (uint32_t)w;
 }
-__device__ __forceinline__ uint32_t pack4f(int fmt, float a, float b, float c, float d) {
-  return fmt == F8_E4M3 ? pack4<F8_E4M3>(a, b, c, d) : pack4<F8_E5M2>(a, b, c, d);
+
+typedef uint64_t u64_any __attribute__((aligned(1)));
+// n <= 8 scale bytes (byte i of w) to p
+__device__ __forceinline__ void put_scales(uint8_t* p, uint64_t w, int n) {
+  if (n >= 8) {
+    *(u64_any*)p = w;
+  } else {
+    for (int i = 0; i < n; ++i) p[i] = (uint8_t)(w >> (8 * i));
+  }
 }
 
 template <typename T, bool VEC>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs p) {
-  constexpr int QT_LD = 128 + 16;   // LDS row of x^T codes (16-B aligned, off the 256-B bank period)
-  __shared__ __attribute__((aligned(16))) uint8_t tbuf[128 * QT_LD];
-  __shared__ uint32_t cmax[4][128];
+  constexpr int QT_LD = 33;         // words
+  __shared__ uint32_t tbuf[128 * QT_LD];
+  __shared__ __attribute__((aligned(16))) uint32_t cmax[4][128];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const int g = t >> 4, j = t & 15;
   const int tiles_c = (p.C + 127) >> 7;
@@ -60,114 +79,161 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs p) {
   const int nr = (int)min((long)128, p.R - r0), nc = (int)min((long)128, p.C - c0);
 
   float v[8][8];
+  auto unpack = [&](int i, const uint4& u) {     // 8 bf16
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 8 * g + i, c = 8 * j;
-    if (r < nr && c < nc) {
-      const T* s = x + (long)r * p.ldx + c;
-      if (VEC && c + 8 <= nc) {
-        if constexpr (sizeof(T) == 2) {
-          const uint4 u = *(const uint4*)s;
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int k = 0; k < 4; ++k) {
+      v[i][2 * k] = __uint_as_float(w[k] << 16);
+      v[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+    }
+  };
+  // all loads are on their way before the first is used; behind the last row or column the last one is loaded again
+  if (32 * wave >= nr) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            v[i][2 * k] = __uint_as_float(w[k] << 16);
-            v[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-          }
-        } else {
-          const f32x4_t a = *(const f32x4_t*)s, b = *(const f32x4_t*)(s + 4);
+    for (int i = 0; i < 64; ++i) (&v[0][0])[i] = 0.f;
+  } else if (VEC && nc % 8 == 0) {
+    const int c = min(8 * j, nc - 8);
+    if constexpr (sizeof(T) == 2) {
+      uint4 u[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) { v[i][k] = a[k]; v[i][4 + k] = b[k]; }
-        }
-      } else {
+      for (int i = 0; i < 8; ++i) u[i] = *(const uint4*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = c + k < nc ? to_f32<T>(s[k]) : 0.f;
-      }
+      for (int i = 0; i < 8; ++i) unpack(i, u[i]);
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const f32x4_t* s = (const f32x4_t*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
+        const f32x4_t a = s[0], b = s[1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { v[i][k] = a[k]; v[i][4 + k] = b[k]; }
+      }
     }
-  }
-
-  uint32_t rowmax[8];
+    if (nr < 128 || nc < 128) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t m = 0;
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, finite_bits(v[i][k]));
-    rowmax[i] = m;
-  }
-  uint32_t tilemax = 0;
-  if (p.tile) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) tilemax = max(tilemax, rowmax[i]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) tilemax = max(tilemax, (uint32_t)__shfl_xor((int)tilemax, d));
-    if (lane == 0) cmax[0][wave] = tilemax;
-    __syncthreads();
-    tilemax = max(max(cmax[0][0], cmax[0][1]), max(cmax[0][2], cmax[0][3]));
-    __syncthreads();
-  }
-
-  if (p.q != nullptr) {
+        for (int k = 0; k < 8; ++k) v[i][k] = 8 * g + i < nr && 8 * j < nc ? v[i][k] : 0.f;
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      uint32_t m = rowmax[i];
-      if (p.tile) {
-        m = tilemax;
-      } else {
+      const T* s = x + (long)min(8 * g + i, nr - 1) * p.ldx;
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-      }
-      const uint32_t b = e8m0_of_amax(m, p.fmt);
-      const float s = e8m0_inv(b);
-      const int r = 8 * g + i;
-      if (r < nr) {
-        uint2 o;
-        o.x = pack4f(p.fmt, v[i][0] * s, v[i][1] * s, v[i][2] * s, v[i][3] * s);
-        o.y = pack4f(p.fmt, v[i][4] * s, v[i][5] * s, v[i][6] * s, v[i][7] * s);
-        *(uint2*)(p.q + (r0 + r) * p.ldq + c0 + 8 * j) = o;
-        if (j == 0) p.sq[(long)tc * p.ldsq + r0 + r] = (uint8_t)b;
-      }
+      for (int k = 0; k < 8; ++k) v[i][k] = to_f32<T>(s[min(8 * j + k, nc - 1)]);
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = 8 * g + i < nr && 8 * j + k < nc ? v[i][k] : 0.f;
   }
 
-  if (p.qt != nullptr) {
-    uint32_t cm[8];
+  // maxima of the thread's rows and columns; where there is an inf or NaN among them, again over the finite elements
+  uint32_t rowmax[8], colmax[8], all = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) cm[k] = tilemax;
-    if (!p.tile) {
+  for (int i = 0; i < 8; ++i) rowmax[i] = colmax[i] = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i += 2)
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {     // 2 x 2 at a time: four magnitudes are alive, not 64
+      const uint32_t m00 = abs_bits(v[i][k]), m01 = abs_bits(v[i][k + 1]), m10 = abs_bits(v[i + 1][k]), m11 = abs_bits(v[i + 1][k + 1]);
+      rowmax[i] = max(max(rowmax[i], m00), m01);
+      rowmax[i + 1] = max(max(rowmax[i + 1], m10), m11);
+      colmax[k] = max(max(colmax[k], m00), m10);
+      colmax[k + 1] = max(max(colmax[k + 1], m01), m11);
+    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) all = max(all, rowmax[i]);
+  if (all >= 0x7f800000u) {
+    all = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      rowmax[i] = colmax[i] = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, finite_bits(v[i][k]));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-        if (lane < 16) cmax[wave][8 * j + k] = m;
+        asm("" : "+v"(v[i][k]));           // (not the magnitudes from above, kept for here)
+        rowmax[i] = max(rowmax[i], finite_bits(v[i][k]));
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int c = 8 * j + k;
-        cm[k] = max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c]));
-      }
+      all = max(all, rowmax[i]);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t b = e8m0_of_amax(cm[k], p.fmt_t);
-      const float s = e8m0_inv(b);
-      uint2 o;
-      o.x = pack4f(p.fmt_t, v[0][k] * s, v[1][k] * s, v[2][k] * s, v[3][k] * s);
-      o.y = pack4f(p.fmt_t, v[4][k] * s, v[5][k] * s, v[6][k] * s, v[7][k] * s);
-      *(uint2*)(tbuf + (8 * j + k) * QT_LD + 8 * g) = o;
-      if (g == 0 && 8 * j + k < nc) p.sqt[(long)tr * p.ldsqt + c0 + 8 * j + k] = (uint8_t)b;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) colmax[k] = max(colmax[k], finite_bits(v[i][k]));
     }
+  }
+  if (p.tile) {
+    all = max_row16(all);
+    all = max(all, (uint32_t)__shfl_xor((int)all, 16));
+    all = max(all, (uint32_t)__shfl_xor((int)all, 32));
+    if (lane == 0) cmax[0][wave] = all;
+    __syncthreads();
+    all = max(max(cmax[0][0], cmax[0][1]), max(cmax[0][2], cmax[0][3]));
+    __syncthreads();
+  }
+
+  using E4 = std::integral_constant<int, F8_E4M3>;
+  using E5 = std::integral_constant<int, F8_E5M2>;
+  if (p.q != nullptr) {
+    auto rows = [&](auto fmt) {
+      uint64_t bytes = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t b = e8m0_of_amax(p.tile ? all : max_row16(rowmax[i]), fmt.value);
+        const float s = e8m0_inv(b);
+        bytes |= (uint64_t)b << (8 * i);
+        const int r = 8 * g + i;
+        uint2 o;
+        o.x = pack4<fmt.value>(v[i][0] * s, v[i][1] * s, v[i][2] * s, v[i][3] * s);
+        o.y = pack4<fmt.value>(v[i][4] * s, v[i][5] * s, v[i][6] * s, v[i][7] * s);
+        if (r < nr) *(uint2*)(p.q + (r0 + r) * p.ldq + c0 + 8 * j) = o;
+      }
+      if (j == 0) put_scales(p.sq + (long)tc * p.ldsq + r0 + 8 * g, bytes, nr - 8 * g);
+    };
+    if (p.fmt == F8_E4M3) rows(E4{});
+    else rows(E5{});
+  }
+
+  if (p.qt != nullptr) {
+    if (!p.tile) {
+      // over the wave's four g: each exchange keeps half of the columns, lane row g % 4 = 2 a + b ends with 4 a + 2 b and the
+      // one after it
+      typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+      uint32_t h[4], q[2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x2_t w = __builtin_amdgcn_permlane32_swap(colmax[k], colmax[4 + k], false, false);
+        h[k] = max(w[0], w[1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const u32x2_t w = __builtin_amdgcn_permlane16_swap(h[k], h[2 + k], false, false);
+        q[k] = max(w[0], w[1]);
+      }
+      *(uint2*)&cmax[wave][8 * j + 4 * (lane >> 5) + 2 * (lane >> 4 & 1)] = uint2{q[0], q[1]};
+      __syncthreads();
+    }
+    auto columns = [&](auto fmt) {
+      uint64_t bytes = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = 8 * j + k;
+        const uint32_t b = e8m0_of_amax(p.tile ? all : max(max(cmax[0][c], cmax[1][c]), max(cmax[2][c], cmax[3][c])), fmt.value);
+        const float s = e8m0_inv(b);
+        bytes |= (uint64_t)b << (8 * k);
+        uint32_t* o = tbuf + c * QT_LD + 2 * g;
+        o[0] = pack4<fmt.value>(v[0][k] * s, v[1][k] * s, v[2][k] * s, v[3][k] * s);
+        o[1] = pack4<fmt.value>(v[4][k] * s, v[5][k] * s, v[6][k] * s, v[7][k] * s);
+      }
+      if (g == 0) put_scales(p.sqt + (long)tr * p.ldsqt + c0 + 8 * j, bytes, nc - 8 * j);
+    };
+    if (p.fmt_t == F8_E4M3) columns(E4{});
+    else columns(E5{});
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = 32 * i + (t >> 3), o = 16 * (t & 7);
-      if (c < nc) *(uint4*)(p.qt + (c0 + c) * p.ldqt + r0 + o) = *(const uint4*)(tbuf + c * QT_LD + o);
+      const int c = 32 * i + (t >> 3), o = t & 7;
+      const uint32_t* w = tbuf + c * QT_LD + 4 * o;
+      if (c < nc) *(uint4*)(p.qt + (c0 + c) * p.ldqt + r0 + 16 * o) = uint4{w[0], w[1], w[2], w[3]};
     }
   }
 }

@@ -56,6 +56,25 @@ def test_quantize_special_values(fmt, tile):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("bits", [0x7f81, 0x7fc0, 0xff80, 0x0001])
+def test_quantize_bit_patterns(dtype, tile, bits):
+    """Signalling and quiet NaN, -inf and the smallest subnormal among ordinary values, in every position of a block's lanes:
+    the block's scale and its other values are those of the CPU form."""
+    x = rand(140, 260, 3, dtype)
+    word = torch.tensor(bits << 16 if dtype == torch.float32 else bits, dtype=torch.int64)
+    i = torch.arange(140)
+    for c in (7, 70, 255):
+        x.view(torch.int32 if dtype == torch.float32 else torch.int16)[i, (i + c) % 260] = \
+            (word - 2 ** 32 if word >= 2 ** 31 else word).to(torch.int32) if dtype == torch.float32 else \
+            (word - 2 ** 16 if word >= 2 ** 15 else word).to(torch.int16)
+    for fmt in ("e4m3", "e5m2"):
+        q, qt = fp8.quantize_fp8_both(x.to(DEV), fmt, fmt, tile=tile)
+        same_operand(q, fp8.quantize_fp8(x, fmt, tile=tile))
+        same_operand(qt, fp8.quantize_fp8_t(x, fmt, tile=tile))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_quantize_strided_and_misaligned(dtype):
     """Column slices (rows off the 16-byte grid), a transposed view, an expanded row, and writes that stay inside out."""
     base = rand(200, 300, 5, dtype)
