@@ -1014,4 +1014,76 @@ int dllm_fp8_gemm(const void* A, long lda, const void* SA, long ldsa, int fa, co
   }
 }
 
+// ---- the linear layer's calls: the quantisations and products of one direction, their temporaries in one workspace ----
+struct LinWs {
+  uint8_t *a, *sa, *b, *sb;    // two quantised operands [ra, pad128(ka)], [rb, pad128(kb)] and their scales
+  float* part;                 // K slices' sums of whichever product runs
+  long bytes;
+};
+static LinWs lin_ws(char* base, long ra, long ka, long rb, long kb, long part) {
+  LinWs w;
+  long o = 0;
+  auto take = [&](long n) {
+    char* p = base + o;
+    o += (n + 255) / 256 * 256;
+    return p;
+  };
+  const long na = (ka + 127) / 128, nb = (kb + 127) / 128;
+  w.a = (uint8_t*)take(ra * na * 128); w.sa = (uint8_t*)take(na * ra);
+  w.b = (uint8_t*)take(rb * nb * 128); w.sb = (uint8_t*)take(nb * rb);
+  w.part = (float*)take(part * 4);
+  w.bytes = o;
+  return w;
+}
+// floats that a product's K slices need
+static long lin_part(int M, int N, int K, int odt) {
+  const int t = dllm_fp8_gemm_plan(M, N, (K + 127) / 128, odt) >> 16;
+  return t > 1 ? (long)t * M * N : 0;
+}
+static int lin_gemm(const uint8_t* A, long lda, const uint8_t* SA, long ldsa, int fa, const uint8_t* B, long ldb,
+                    const uint8_t* SB, long ldsb, int fb, void* C, long ldc, int odt, int M, int N, int K, float beta, float* part,
+                    void* stream) {
+  const int nk = (K + 127) / 128, t = dllm_fp8_gemm_plan(M, N, nk, odt);
+  return dllm_fp8_gemm(A, lda, SA, ldsa, fa, B, ldb, SB, ldsb, fb, C, ldc, odt, nullptr, nullptr, 0, M, N, nk, 1.f, beta, EPI_STORE,
+                       ACT_NONE, t & 0xffff, t >> 16, part, stream);
+}
+
+// bytes of workspace of dllm_linear_fp8 (y of type odt) and of dllm_linear_fp8_bwd (dx, dw of types dxdt, dwdt)
+long dllm_linear_fp8_workspace(int T, int D, int F, int odt) { return lin_ws(nullptr, T, D, F, D, lin_part(T, F, D, odt)).bytes; }
+long dllm_linear_fp8_bwd_workspace(int T, int D, int F, int dxdt, int dwdt) {
+  return lin_ws(nullptr, T, F, F, T, max(lin_part(T, D, F, dxdt), lin_part(F, D, T, dwdt))).bytes;
+}
+
+// y [T, F] = x [T, D] w [F, D]^T; leaves x^T [D, T] and w^T [D, F] in 8 bits (rows of pad128 codes, dense scales)
+int dllm_linear_fp8(const void* x, int xdt, long ldx, const void* w, int wdt, long ldw, int T, int D, int F, void* xt, void* sxt,
+                    void* wt, void* swt, void* y, int odt, long ldy, void* ws, long ws_bytes, void* stream) {
+  if (T <= 0 || D <= 0 || F <= 0 || (odt != DT_BF16 && odt != DT_F32)) return -1;
+  const LinWs l = lin_ws((char*)ws, T, D, F, D, lin_part(T, F, D, odt));
+  if (ws == nullptr || (uintptr_t)ws % 256 || ws_bytes < l.bytes) return -1;
+  const long pd = ((long)D + 127) / 128 * 128, pt = ((long)T + 127) / 128 * 128, pf = ((long)F + 127) / 128 * 128;
+  int rc = dllm_fp8_quantize(x, xdt, ldx, T, D, l.a, pd, l.sa, T, xt, pt, sxt, D, F8_E4M3, F8_E4M3, 0, stream);
+  if (rc == 0) rc = dllm_fp8_quantize(w, wdt, ldw, F, D, l.b, pd, l.sb, F, wt, pf, swt, D, F8_E4M3, F8_E4M3, 1, stream);
+  if (rc == 0) rc = lin_gemm(l.a, pd, l.sa, T, F8_E4M3, l.b, pd, l.sb, F, F8_E4M3, y, ldy, odt, T, F, D, 0.f, l.part, stream);
+  return rc;
+}
+
+// dx [T, D] = dy [T, F] w (skipped where dx is null), dw [F, D] = dy^T x + beta dw, from dy in e5m2
+int dllm_linear_fp8_bwd(const void* dy, int ydt, long ldy, int T, int D, int F, const void* xt, long ldxt, const void* sxt,
+                        long ldsxt, int fx, const void* wt, long ldwt, const void* swt, long ldswt, int fw, void* dx, int dxdt,
+                        long lddx, void* dw, int dwdt, long lddw, float beta, void* ws, long ws_bytes, void* stream) {
+  if (T <= 0 || D <= 0 || F <= 0 || (dwdt != DT_BF16 && dwdt != DT_F32) || (dxdt != DT_BF16 && dxdt != DT_F32)) return -1;
+  const LinWs l = lin_ws((char*)ws, T, F, F, T, max(lin_part(T, D, F, dxdt), lin_part(F, D, T, dwdt)));
+  if (ws == nullptr || (uintptr_t)ws % 256 || ws_bytes < l.bytes || dw == nullptr) return -1;
+  const long pt = ((long)T + 127) / 128 * 128, pf = ((long)F + 127) / 128 * 128;
+  int rc = dllm_fp8_quantize(dy, ydt, ldy, T, F, dx ? l.a : nullptr, pf, dx ? l.sa : nullptr, T, l.b, pt, l.sb, F, F8_E5M2, F8_E5M2, 0,
+                             stream);
+  if (rc == 0 && dx)
+    rc = lin_gemm(l.a, pf, l.sa, T, F8_E5M2, (const uint8_t*)wt, ldwt, (const uint8_t*)swt, ldswt, fw, dx, lddx, dxdt, T, D, F, 0.f,
+                  l.part, stream);
+  if (rc == 0)
+    rc = lin_gemm(l.b, pt, l.sb, F, F8_E5M2, (const uint8_t*)xt, ldxt, (const uint8_t*)sxt, ldsxt, fx, dw, lddw, dwdt, F, D, T, beta,
+                  l.part, stream);
+  return rc;
+}
+
 }  // extern "C"

@@ -339,27 +339,104 @@ class LinearFP8(NamedTuple):
     w_t: BlockFP8
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(T: int, D: int, F: int, *codes: int) -> int:
+    f = _native.lib().dllm_linear_fp8_workspace if len(codes) == 1 else _native.lib().dllm_linear_fp8_bwd_workspace
+    return f(T, D, F, *codes)
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.shape[1] <= 1 or x.stride(1) == 1 else x.contiguous()
+
+
 def linear_fp8(x: torch.Tensor, w: torch.Tensor, out: torch.Tensor | None = None,
                out_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, LinearFP8]:
     """``y = x·wᵀ`` (``linear_fwd`` train_ffns.py:41-42) with x [T, D] quantised per row and 128 columns and w [F, D] per
-    128x128 tile, both e4m3.  Returns ``(y, saved)``; ``saved`` goes to ``linear_fp8_bwd``."""
+    128x128 tile, both e4m3.  Returns ``(y, saved)``; ``saved`` goes to ``linear_fp8_bwd``.  The same values as
+    ``quantize_fp8_both`` and ``gemm_fp8`` give, in one call."""
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"linear_fp8: x [T, D] and w [F, D], got {tuple(x.shape)} and {tuple(w.shape)}")
-    xq, xt = quantize_fp8_both(x)
-    wq, wt = quantize_fp8_both(w, tile=True)
-    return gemm_fp8(xq, wq, out, out_dtype=out_dtype), LinearFP8(xt, wt)
+    (T, D), (F, _) = _shape2(x), _shape2(w)
+    dev = x.device
+    if w.device != dev:
+        raise ValueError(f"linear_fp8: x on {dev}, w on {w.device}")
+    if not x.is_cuda or T == 0 or D == 0 or F == 0:
+        xq, xt = quantize_fp8_both(x)
+        wq, wt = quantize_fp8_both(w, tile=True)
+        return gemm_fp8(xq, wq, out, out_dtype=out_dtype), LinearFP8(xt, wt)
+    if out is None:
+        out, ldo = torch.empty((T, F), dtype=out_dtype, device=dev), F
+    else:
+        _check_rows(out, "out", (T, F), dev)
+        ldo, out_dtype = _ld(out), out.dtype
+    oc = _native.DT.get(out_dtype)
+    if oc is None:
+        raise TypeError(f"linear_fp8: out must be bf16 or fp32, got {out_dtype}")
+    x, w = _rows(x), _rows(w)
+    n = _linear_workspace(T, D, F, oc)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    xt, wt = fp8_empty(D, T, "e4m3", dev), fp8_empty(D, F, "e4m3", dev)
+    with _on(dev):
+        rc = _native.lib().dllm_linear_fp8(
+            x.data_ptr(), _native.DT[x.dtype], x.stride(0), w.data_ptr(), _native.DT[w.dtype], w.stride(0), T, D, F,
+            xt.data.data_ptr(), xt.scale.data_ptr(), wt.data.data_ptr(), wt.scale.data_ptr(), out.data_ptr(), oc, ldo,
+            ws.data_ptr(), n, _native.stream_ptr(dev))
+    if rc:
+        _native.check(rc, f"dllm_linear_fp8(T={T},D={D},F={F})")
+    return out, LinearFP8(xt, wt)
 
 
 def linear_fp8_bwd(dy: torch.Tensor, saved: LinearFP8, dw: torch.Tensor | None = None, *, beta: float = 0.0,
                    dx: torch.Tensor | None = None, need_dx: bool = True) -> tuple[torch.Tensor | None, torch.Tensor]:
     """``(dx, dw) = (dy·w, dyᵀ·x)`` (``t_linear_bkwd`` train_ffns.py:44-45) with dy [T, F] quantised to e5m2 (gradients
-    need range more than digits): per row for dx, per column for dw.  ``dx`` has dy's type, ``dw`` is fp32 unless given;
-    ``beta`` accumulates into ``dw``."""
-    if dy.dim() != 2 or dy.shape != (saved.x_t.k, saved.w_t.k):
-        raise ValueError(f"linear_fp8_bwd: dy must be {(saved.x_t.k, saved.w_t.k)}, got {tuple(dy.shape)}")
-    if need_dx:
-        dq, dt = quantize_fp8_both(dy, "e5m2", "e5m2")
-        dx = gemm_fp8(dq, saved.w_t, dx, out_dtype=dy.dtype)
-    else:
-        dx, dt = None, quantize_fp8_t(dy, "e5m2")
-    return dx, gemm_fp8(dt, saved.x_t, dw, out_dtype=torch.float32, beta=beta)
+    need range more than digits): per row for dx, per column for dw.  ``dx`` has dy's type unless given, ``dw`` is fp32
+    unless given; ``beta`` accumulates into ``dw``."""
+    xt, wt = saved
+    T, F, D = xt.k, wt.k, xt.rows
+    if dy.dim() != 2 or dy.shape != (T, F):
+        raise ValueError(f"linear_fp8_bwd: dy must be {(T, F)}, got {tuple(dy.shape)}")
+    if dw is None and beta != 0.0:
+        raise ValueError("linear_fp8_bwd: beta needs dw")
+    if not need_dx and dx is not None:
+        raise ValueError("linear_fp8_bwd: dx given with need_dx = False")
+    _shape2(dy)
+    dev = dy.device
+    if not dy.is_cuda or T == 0 or D == 0 or F == 0:
+        if need_dx:
+            dq, dt = quantize_fp8_both(dy, "e5m2", "e5m2")
+            dx = gemm_fp8(dq, wt, dx, out_dtype=dy.dtype)
+        else:
+            dt = quantize_fp8_t(dy, "e5m2")
+        return dx, gemm_fp8(dt, xt, dw, out_dtype=torch.float32, beta=beta)
+    xarg, warg = _check(xt, "saved.x_t"), _check(wt, "saved.w_t")
+    if xt.device != dev or wt.device != dev or wt.rows != D:
+        raise ValueError(f"linear_fp8_bwd: saved operands {xt.rows} x {T} on {xt.device}, {wt.rows} x {F} on {wt.device} "
+                         f"for dy on {dev}")
+    codes, args = [], []
+    for t, name, shape, dtype in ((dx, "dx", (T, D), dy.dtype), (dw, "dw", (F, D), torch.float32)):
+        if name == "dx" and not need_dx:
+            codes.append(0)
+            args += [None, 0, 0]
+            continue
+        if t is None:
+            t, ld = torch.empty(shape, dtype=dtype, device=dev), D
+        else:
+            _check_rows(t, name, shape, dev)
+            ld, dtype = _ld(t), t.dtype
+        if dtype not in _native.DT:
+            raise TypeError(f"linear_fp8_bwd: {name} must be bf16 or fp32, got {dtype}")
+        codes.append(_native.DT[dtype])
+        args += [t.data_ptr(), codes[-1], ld]
+        if name == "dx":
+            dx = t
+        else:
+            dw = t
+    dy = _rows(dy)
+    n = _linear_workspace(T, D, F, *codes)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = _native.lib().dllm_linear_fp8_bwd(dy.data_ptr(), _native.DT[dy.dtype], dy.stride(0), T, D, F, *xarg, *warg, *args,
+                                               beta, ws.data_ptr(), n, _native.stream_ptr(dev))
+    if rc:
+        _native.check(rc, f"dllm_linear_fp8_bwd(T={T},D={D},F={F})")
+    return dx, dw

@@ -214,5 +214,9 @@ def test_refusals():
     with pytest.raises(ValueError, match="x \\[T, D\\]"):
         fp8.linear_fp8(torch.randn(3, 4), torch.randn(5, 6))
     _, saved = fp8.linear_fp8(torch.randn(3, 4), torch.randn(5, 4))
+    y, saved = fp8.linear_fp8(torch.randn(3, 5), torch.randn(7, 5))
+    for kw in ({"beta": 1.0}, {"dx": torch.empty(3, 5), "need_dx": False}):
+        with pytest.raises(ValueError, match="beta needs dw|need_dx"):
+            fp8.linear_fp8_bwd(y.float(), saved, **kw)
     with pytest.raises(ValueError, match="dy must be"):
         fp8.linear_fp8_bwd(torch.randn(3, 4), saved)

@@ -264,6 +264,52 @@ def test_linear(T, D, F):
     product_check(acc, fp8.quantize_fp8_t(dy, "e5m2"), fp8.quantize_fp8_t(x), beta=1.0, c=dw)
 
 
+@pytest.mark.parametrize("T,D,F", [(1, 40, 33), (5, 1, 700), (333, 257, 129), (60, 2048, 4096), (1000, 512, 1400)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_linear_is_its_operators(T, D, F, dtype):
+    """One call per direction, the bits of the separate calls; views in and out, either result type, no input gradient."""
+    big = rand(T, D + 3, 1, dtype).to(DEV)
+    x, w, dy = big[:, 1:D + 1], rand(D, F, 2, dtype).to(DEV).t(), rand(T, F, 3, dtype).to(DEV)
+    xq, xt = fp8.quantize_fp8_both(x)
+    wq, wt = fp8.quantize_fp8_both(w, tile=True)
+    dq, dt = fp8.quantize_fp8_both(dy, "e5m2", "e5m2")
+    for out in (torch.bfloat16, torch.float32):
+        ybuf = torch.full((T, F + 5), 7.0, dtype=out, device=DEV)
+        y, saved = fp8.linear_fp8(x, w, ybuf[:, 2:F + 2])
+        assert torch.equal(y, fp8.gemm_fp8(xq, wq, out_dtype=out)) and (ybuf[:, :2] == 7).all() and (ybuf[:, F + 2:] == 7).all()
+        same_operand(saved.x_t, fp8.BlockFP8(xt.data.cpu(), xt.scale.cpu(), T))
+        same_operand(saved.w_t, fp8.BlockFP8(wt.data.cpu(), wt.scale.cpu(), F))
+        acc = torch.ones(F, D, dtype=out, device=DEV)
+        dx, dw = fp8.linear_fp8_bwd(dy, saved, acc, beta=0.5, dx=torch.empty(T, D, dtype=out, device=DEV))
+        assert torch.equal(dx, fp8.gemm_fp8(dq, wt, out_dtype=out)) and dw is acc
+        assert torch.equal(dw, fp8.gemm_fp8(dt, xt, torch.ones(F, D, dtype=out, device=DEV), beta=0.5))
+    none, dw = fp8.linear_fp8_bwd(dy, saved, need_dx=False)
+    assert none is None and torch.equal(dw, fp8.gemm_fp8(dt, xt, out_dtype=torch.float32))
+
+
+def test_linear_captured_and_replayed():
+    x, w, dy = (rand(r, c, i, torch.bfloat16).to(DEV) for i, (r, c) in enumerate(((200, 300), (500, 300), (200, 500))))
+
+    def step():
+        y, saved = fp8.linear_fp8(x, w)
+        return (y, *fp8.linear_fp8_bwd(dy, saved))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        x.copy_(rand(200, 300, 20 + i))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_other_stream_and_graph():
     """The same bits on another stream, from a captured graph on replayed new inputs, and from the batch-size-one slice."""
     x, w = rand(300, 400, 1, torch.bfloat16).to(DEV), rand(200, 400, 2, torch.bfloat16).to(DEV)
