@@ -10,6 +10,10 @@ typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 
+// 16-byte accesses at any element's address: the hardware takes them unaligned, so odd row lengths need no other path
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+
 // ----------------------------------------------------------------------------------------------
 // quantiser: one block of 256 threads per 128x128 tile of x, one read of x for both orientations
 //
@@ -65,7 +69,7 @@ __device__ __forceinline__ void put_scales(uint8_t* p, uint64_t w, int n) {
   }
 }
 
-template <typename T, bool VEC>
+template <typename T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs p) {
   constexpr int QT_LD = 33;         // words
   __shared__ uint32_t tbuf[128 * QT_LD];
@@ -79,8 +83,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs p) {
   const int nr = (int)min((long)128, p.R - r0), nc = (int)min((long)128, p.C - c0);
 
   float v[8][8];
-  auto unpack = [&](int i, const uint4& u) {     // 8 bf16
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  auto unpack = [&](int i, const u32x4_any& w) {     // 8 bf16
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       v[i][2 * k] = __uint_as_float(w[k] << 16);
@@ -91,18 +94,18 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(QuantArgs p) {
   if (32 * wave >= nr) {
 #pragma unroll
     for (int i = 0; i < 64; ++i) (&v[0][0])[i] = 0.f;
-  } else if (VEC && nc % 8 == 0) {
+  } else if (nc % 8 == 0) {
     const int c = min(8 * j, nc - 8);
     if constexpr (sizeof(T) == 2) {
-      uint4 u[8];
+      u32x4_any u[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = *(const uint4*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
+      for (int i = 0; i < 8; ++i) u[i] = *(const u32x4_any*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
 #pragma unroll
       for (int i = 0; i < 8; ++i) unpack(i, u[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const f32x4_t* s = (const f32x4_t*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
+        const f32x4_any* s = (const f32x4_any*)(x + (long)min(8 * g + i, nr - 1) * p.ldx + c);
         const f32x4_t a = s[0], b = s[1];
 #pragma unroll
         for (int k = 0; k < 4; ++k) { v[i][k] = a[k]; v[i][4 + k] = b[k]; }
@@ -259,15 +262,15 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* q, l
       v[4 * h] = a[0] * s; v[4 * h + 1] = a[1] * s; v[4 * h + 2] = b[0] * s; v[4 * h + 3] = b[1] * s;
     }
     T* o = out + r * ldo + c;
-    if (c + 8 <= K && (((uintptr_t)o) & 15) == 0) {
+    if (c + 8 <= K) {
       if constexpr (sizeof(T) == 2) {
-        uint4 u;
+        u32x4_any u;
         u.x = f2bf(v[0]) | ((uint32_t)f2bf(v[1]) << 16); u.y = f2bf(v[2]) | ((uint32_t)f2bf(v[3]) << 16);
         u.z = f2bf(v[4]) | ((uint32_t)f2bf(v[5]) << 16); u.w = f2bf(v[6]) | ((uint32_t)f2bf(v[7]) << 16);
-        *(uint4*)o = u;
+        *(u32x4_any*)o = u;
       } else {
-        *(f32x4_t*)o = f32x4_t{v[0], v[1], v[2], v[3]};
-        *(f32x4_t*)(o + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        *(f32x4_any*)o = f32x4_any{v[0], v[1], v[2], v[3]};
+        *(f32x4_any*)(o + 4) = f32x4_any{v[4], v[5], v[6], v[7]};
       }
     } else {
       for (int k = 0; k < 8 && c + k < K; ++k) {
@@ -334,12 +337,6 @@ __device__ __forceinline__ void f8_epi1(const Fp8GemmArgs& p, int m, int n, floa
     o *= act_grad(p.act, ld_out<OutT>(p.aux, ia));
   }
   st_out<OutT>(p.C, i, o);
-}
-// whether rows of C and aux take 16-byte accesses
-template <typename OutT>
-__device__ __forceinline__ bool f8_aligned(const Fp8GemmArgs& p) {
-  return p.ldc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && p.ldaux % 8 == 0 && (uintptr_t)p.aux % 16 == 0 &&
-         (uintptr_t)p.aux_out % 16 == 0;
 }
 
 // ----------------------------------------------------------------------------------------------
@@ -466,40 +463,41 @@ struct F8Trait {
   }
 };
 
-// 8 columns n .. n + 7 of row m; `fast`: the tile is inside C and rows are 16-byte aligned
+// 8 columns n .. n + 7 of row m; `inside`: the whole tile is inside C
 template <int EPI, typename OutT>
-__device__ __forceinline__ void f8_epi8(const Fp8GemmArgs& p, bool fast, int m, int n, const float (&v)[8]) {
-  if (!fast) {
-    if (m < p.M)
+__device__ __forceinline__ void f8_epi8(const Fp8GemmArgs& p, bool inside, int m, int n, const float (&v)[8]) {
+  if (!inside) {
+    if (m >= p.M) return;
+    if (n + 8 > p.N) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (n + e < p.N) f8_epi1<EPI, OutT>(p, m, n + e, v[e]);
-    return;
+      return;
+    }
   }
   auto load = [](const void* base, long i, float (&x)[8]) {
     if constexpr (sizeof(OutT) == 2) {
-      const uint4 u = *(const uint4*)((const uint16_t*)base + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      const u32x4_any w = *(const u32x4_any*)((const uint16_t*)base + i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         x[2 * k] = __uint_as_float(w[k] << 16);
         x[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
       }
     } else {
-      const f32x4_t a = *(const f32x4_t*)((const float*)base + i), b = *(const f32x4_t*)((const float*)base + i + 4);
+      const f32x4_any a = *(const f32x4_any*)((const float*)base + i), b = *(const f32x4_any*)((const float*)base + i + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) { x[k] = a[k]; x[4 + k] = b[k]; }
     }
   };
   auto store = [](void* base, long i, const float (&x)[8]) {
     if constexpr (sizeof(OutT) == 2) {
-      uint4 u;
+      u32x4_any u;
       u.x = f2bf(x[0]) | ((uint32_t)f2bf(x[1]) << 16); u.y = f2bf(x[2]) | ((uint32_t)f2bf(x[3]) << 16);
       u.z = f2bf(x[4]) | ((uint32_t)f2bf(x[5]) << 16); u.w = f2bf(x[6]) | ((uint32_t)f2bf(x[7]) << 16);
-      *(uint4*)((uint16_t*)base + i) = u;
+      *(u32x4_any*)((uint16_t*)base + i) = u;
     } else {
-      *(f32x4_t*)((float*)base + i) = f32x4_t{x[0], x[1], x[2], x[3]};
-      *(f32x4_t*)((float*)base + i + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
+      *(f32x4_any*)((float*)base + i) = f32x4_any{x[0], x[1], x[2], x[3]};
+      *(f32x4_any*)((float*)base + i + 4) = f32x4_any{x[4], x[5], x[6], x[7]};
     }
   };
   const long i = (long)m * p.ldc + n, ia = (long)m * p.ldaux + n;
@@ -550,7 +548,7 @@ __global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
   for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   n8_loop(tr, lds, (const char*)p.A + (long)m0 * p.lda, (const char*)p.B + (long)n0 * p.ldb, tr.step(0), ao, bo, tr.nk2, wid,
           lane, acc);
-  const bool fast = left_m == 255 && left_n == 255 && f8_aligned<OutT>(p);
+  const bool inside = left_m == 255 && left_n == 255;
 #pragma unroll
   for (int qm = 0; qm < 2; ++qm)
 #pragma unroll
@@ -560,7 +558,7 @@ __global__ __launch_bounds__(512, 2) void fp8_gemm_256(Fp8GemmArgs p) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = acc[qm][qn][mt][e & 1][e >> 1];
-        f8_epi8<EPI, OutT>(p, fast, m0 + n8_row(wid, lane, qm, mt), n0 + n8_col(wid, lane, qn), v);
+        f8_epi8<EPI, OutT>(p, inside, m0 + n8_row(wid, lane, qm, mt), n0 + n8_col(wid, lane, qn), v);
       }
 }
 
@@ -700,7 +698,7 @@ __device__ __forceinline__ void fp8_w4_body(const Fp8GemmArgs& p, DLLM_LDS char*
 
   // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
   const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
-  const bool fast = f8_aligned<OutT>(p) && n0 + TS <= p.N && m0 + TS <= p.M;
+  const bool inside = n0 + TS <= p.N && m0 + TS <= p.M;
 #pragma unroll
   for (int i = 0; i < F; ++i)
 #pragma unroll
@@ -712,12 +710,17 @@ __device__ __forceinline__ void fp8_w4_body(const Fp8GemmArgs& p, DLLM_LDS char*
         const int m = mb + i, n = nb + 8 * c8;
         if (m < p.M) {
           float* o = p.ws + (long)blockIdx.y * p.M * p.N + (long)m * p.N + n;
+          if (n + 8 <= p.N) {
+            *(f32x4_any*)o = f32x4_any{v[0], v[1], v[2], v[3]};
+            *(f32x4_any*)(o + 4) = f32x4_any{v[4], v[5], v[6], v[7]};
+          } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e < p.N) o[e] = v[e];
+            for (int e = 0; e < 8; ++e)
+              if (n + e < p.N) o[e] = v[e];
+          }
         }
       } else {
-        f8_epi8<EPI, OutT>(p, fast, mb + i, nb + 8 * c8, v);
+        f8_epi8<EPI, OutT>(p, inside, mb + i, nb + 8 * c8, v);
       }
     }
 }
@@ -943,17 +946,10 @@ int dllm_fp8_quantize(const void* x, int dtype, long ldx, int R, int C, void* q,
   if (q && (sq == nullptr || ldq < cb * 128 || ldq % 16 || (uintptr_t)q % 16 || ldsq < R)) return -1;
   if (qt && (sqt == nullptr || ldqt < rb * 128 || ldqt % 16 || (uintptr_t)qt % 16 || ldsqt < C)) return -1;
   QuantArgs p{x, ldx, R, C, (uint8_t*)q, ldq, (uint8_t*)sq, ldsq, (uint8_t*)qt, ldqt, (uint8_t*)sqt, ldsqt, fmt, fmt_t, tile};
-  const int es = dtype == DT_BF16 ? 2 : 4;
-  const bool vec = (uintptr_t)x % 16 == 0 && (ldx * es) % 16 == 0;
   const dim3 grid((unsigned)(rb * cb)), block(256);
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == DT_BF16) {
-    if (vec) hipLaunchKernelGGL((fp8_quantize_kernel<uint16_t, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((fp8_quantize_kernel<uint16_t, false>), grid, block, 0, s, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((fp8_quantize_kernel<float, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((fp8_quantize_kernel<float, false>), grid, block, 0, s, p);
-  }
+  if (dtype == DT_BF16) hipLaunchKernelGGL(fp8_quantize_kernel<uint16_t>, grid, block, 0, s, p);
+  else hipLaunchKernelGGL(fp8_quantize_kernel<float>, grid, block, 0, s, p);
   return (int)hipGetLastError();
 }
 

@@ -28,6 +28,8 @@ namespace dllm {
 typedef _Float16 f16;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4_t;
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));   // unaligned 16-byte accesses
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr int SX = 15, SA = 15, SP = 14, SQ = 10;   // plane scales 2^s of X, A (and P A), P, products of P
@@ -69,23 +71,20 @@ __device__ __forceinline__ float muon_u(const MuonIn& p, long i) {
   return p.nesterov ? fmaf(p.beta, m, p.gscale * ld_g(p, i)) : m;
 }
 
-// four elements of g / the momentum at i (VEC: 16-byte aligned fp32, 8-byte aligned bf16; else one at a time)
-template <bool VEC>
+// four elements of g / of u at i
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 __device__ __forceinline__ f32x4_t ld_g4(const MuonIn& p, long i) {
-  if constexpr (!VEC) return f32x4_t{ld_g(p, i), ld_g(p, i + 1), ld_g(p, i + 2), ld_g(p, i + 3)};
-  if (p.gdt != DT_BF16) return *(const f32x4_t*)((const float*)p.g + i);
-  const uint2 w = *(const uint2*)((const uint16_t*)p.g + i);
+  if (p.gdt != DT_BF16) return *(const f32x4_any*)((const float*)p.g + i);
+  const u32x2_any w = *(const u32x2_any*)((const uint16_t*)p.g + i);
   return f32x4_t{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
                  __uint_as_float(w.y & 0xffff0000u)};
 }
-template <int KIND, bool VEC>
+template <int KIND>
 __device__ __forceinline__ f32x4_t muon_u4(const MuonIn& p, long i) {
-  if constexpr (KIND == NS_ORTH) return ld_g4<VEC>(p, i);
-  f32x4_t m;
-  if constexpr (VEC) m = *(const f32x4_t*)(p.mom + i);
-  else m = f32x4_t{p.mom[i], p.mom[i + 1], p.mom[i + 2], p.mom[i + 3]};
+  if constexpr (KIND == NS_ORTH) return ld_g4(p, i);
+  const f32x4_t m = *(const f32x4_any*)(p.mom + i);
   if (!p.nesterov) return m;
-  const f32x4_t g = ld_g4<VEC>(p, i);
+  const f32x4_t g = ld_g4(p, i);
   f32x4_t u;
 #pragma unroll
   for (int k = 0; k < 4; ++k) u[k] = fmaf(p.beta, m[k], p.gscale * g[k]);
@@ -94,27 +93,27 @@ __device__ __forceinline__ f32x4_t muon_u4(const MuonIn& p, long i) {
 
 // momentum update and the partial sums of u^2 (64-bit: gradients of any magnitude, and a sum that does not depend on how it
 // is cut).  grid (NS_PARTS, B).  Bound by HBM: one read of g (and of the momentum, and its write)
-template <int KIND, bool VEC>
+template <int KIND>
 __device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, int z, long n) {
   double s = 0.0;
-  const long chunk = (long)p.il * p.C;                       // contiguous elements of one matrix
+  const long chunk = (long)p.il * p.C;                       // contiguous elements of one matrix (0: all)
   auto at = [&](long i) { return p.il ? (i / chunk * p.B + z) * chunk + i % chunk : (long)z * n + i; };
-  const long n4 = VEC ? n >> 2 : 0, stride = (long)gridDim.x * blockDim.x, t0 = (long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long n4 = chunk % 4 == 0 ? n >> 2 : 0, stride = (long)gridDim.x * blockDim.x, t0 = (long)blockIdx.x * blockDim.x + threadIdx.x;
 #pragma unroll 4
   for (long j = t0; j < n4; j += stride) {
     const long i = at(4 * j);
     if constexpr (KIND == NS_MUON) {
-      const f32x4_t g = ld_g4<VEC>(p, i);
-      f32x4_t m = *(const f32x4_t*)(p.mom + i);
+      const f32x4_t g = ld_g4(p, i);
+      f32x4_t m = *(const f32x4_any*)(p.mom + i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         m[k] = fmaf(p.beta, m[k], p.gscale * g[k]);
         const double u = (double)(p.nesterov ? fmaf(p.beta, m[k], p.gscale * g[k]) : m[k]);
         s += u * u;
       }
-      *(f32x4_t*)(p.mom + i) = m;
+      *(f32x4_any*)(p.mom + i) = m;
     } else {
-      const f32x4_t u = ld_g4<VEC>(p, i);
+      const f32x4_t u = ld_g4(p, i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) s += (double)u[k] * (double)u[k];
     }
@@ -127,21 +126,11 @@ __device__ __forceinline__ double muon_sumsq_part(const MuonIn& p, int z, long n
   }
   return s;
 }
-// whether the matrix that starts at element `base` takes the 16-byte accesses
-template <int KIND>
-__device__ __forceinline__ bool muon_vec(const MuonIn& p, long base) {
-  const uintptr_t g = (uintptr_t)p.g + (uintptr_t)base * (p.gdt == DT_BF16 ? 2 : 4);
-  return g % 16 == 0 && (KIND == NS_ORTH || (uintptr_t)(p.mom + base) % 16 == 0);
-}
-
 template <int KIND>
 __global__ __launch_bounds__(1024) void muon_sumsq_kernel(MuonIn p, double* part) {
   __shared__ double red[16];
   const int z = blockIdx.y;
-  const long n = (long)p.R * p.C, base = muon_row(p.il, p.B, p.R, p.C, z, 0);
-  // (alternating rows: whole vectors in every block of rows)
-  const bool vec = muon_vec<KIND>(p, base) && (p.il == 0 || p.il * (long)p.C % 8 == 0);
-  double s = vec ? muon_sumsq_part<KIND, true>(p, z, n) : muon_sumsq_part<KIND, false>(p, z, n);
+  double s = muon_sumsq_part<KIND>(p, z, (long)p.R * p.C);
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -173,15 +162,14 @@ __global__ __launch_bounds__(256) void ns_split_kernel(MuonIn p, const double* p
   f16* so = same + (long)blockIdx.z * 2 * plane;
   f16* to = tr + (long)blockIdx.z * 2 * plane;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, q = t >> 4, j = 4 * (t & 15);
-  const bool vec = p.C % 8 == 0 && muon_vec<KIND>(p, 0);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = r0 + 16 * i + q, c = c0 + j;
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     if (r < p.R && c < p.C) {
       const long o = muon_row(p.il, p.B, p.R, p.C, blockIdx.z, r) + c;
-      if (vec) {
-        v = muon_u4<KIND, true>(p, o);
+      if (c + 4 <= p.C) {
+        v = muon_u4<KIND>(p, o);
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -230,7 +218,7 @@ struct NsGemm {
   f16* out; long ldo, po, bo;          // planes (NS_PLANES / NS_PLANES_T / NS_POLY)
   f16* outT; long ldt, pt, bt;         // transposed planes (NS_PLANES_T)
   const f16* aux; float cb, ca;        // NS_POLY: A's planes (out's layout), b's factor, a on the diagonal
-  void* C; int cdt, R, Cc, vec;        // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
+  void* C; int cdt, R, Cc;             // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
   int il, nb;                          // NS_STEP: alternating rows, as in MuonIn
   float* w; uint16_t* copy; int16_t* lo; float decay, rate;   // NS_STEP: fp32 master (+ bf16 copy), or split (lo, copy)
   int sym;                             // the product is symmetric: tiles on and below the diagonal, mirrored on writing
@@ -241,19 +229,19 @@ template <int EPI>
 __device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n, const float (&v)[8]) {
   if (m >= p.R || n >= p.Cc) return;
   const long o = muon_row(p.il, p.nb, p.R, p.Cc, z, m) + n;
-  if (p.vec) {   // whole rows of 8, 16-byte aligned
+  if (n + 8 <= p.Cc) {   // 16-byte accesses at any element's address
     if constexpr (EPI == NS_OUT) {
       if (p.cdt == DT_BF16) {
-        uint4 u;
+        u32x4_any u;
         u.x = f2bf(p.cs * v[0]) | (uint32_t)f2bf(p.cs * v[1]) << 16; u.y = f2bf(p.cs * v[2]) | (uint32_t)f2bf(p.cs * v[3]) << 16;
         u.z = f2bf(p.cs * v[4]) | (uint32_t)f2bf(p.cs * v[5]) << 16; u.w = f2bf(p.cs * v[6]) | (uint32_t)f2bf(p.cs * v[7]) << 16;
-        *(uint4*)((uint16_t*)p.C + o) = u;
+        *(u32x4_any*)((uint16_t*)p.C + o) = u;
       } else {
-        *(f32x4_t*)((float*)p.C + o) = f32x4_t{p.cs * v[0], p.cs * v[1], p.cs * v[2], p.cs * v[3]};
-        *(f32x4_t*)((float*)p.C + o + 4) = f32x4_t{p.cs * v[4], p.cs * v[5], p.cs * v[6], p.cs * v[7]};
+        *(f32x4_any*)((float*)p.C + o) = f32x4_any{p.cs * v[0], p.cs * v[1], p.cs * v[2], p.cs * v[3]};
+        *(f32x4_any*)((float*)p.C + o + 4) = f32x4_any{p.cs * v[4], p.cs * v[5], p.cs * v[6], p.cs * v[7]};
       }
     } else if (p.lo != nullptr) {
-      const uint4 wh = *(const uint4*)(p.copy + o), wl = *(const uint4*)((const uint16_t*)p.lo + o);
+      const u32x4_any wh = *(const u32x4_any*)(p.copy + o), wl = *(const u32x4_any*)((const uint16_t*)p.lo + o);
       uint32_t h[4] = {wh.x, wh.y, wh.z, wh.w}, l[4] = {wl.x, wl.y, wl.z, wl.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -261,22 +249,22 @@ __device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n,
         split_join2(h[k], l[k], a, b);
         split_part2(fmaf(-p.rate, p.cs * v[2 * k], a * p.decay), fmaf(-p.rate, p.cs * v[2 * k + 1], b * p.decay), h[k], l[k]);
       }
-      *(uint4*)(p.copy + o) = uint4{h[0], h[1], h[2], h[3]};
-      *(uint4*)((uint16_t*)p.lo + o) = uint4{l[0], l[1], l[2], l[3]};
+      *(u32x4_any*)(p.copy + o) = u32x4_any{h[0], h[1], h[2], h[3]};
+      *(u32x4_any*)((uint16_t*)p.lo + o) = u32x4_any{l[0], l[1], l[2], l[3]};
     } else {
-      f32x4_t a = *(const f32x4_t*)(p.w + o), b = *(const f32x4_t*)(p.w + o + 4);
+      f32x4_any a = *(const f32x4_any*)(p.w + o), b = *(const f32x4_any*)(p.w + o + 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         a[k] = fmaf(-p.rate, p.cs * v[k], a[k] * p.decay);
         b[k] = fmaf(-p.rate, p.cs * v[4 + k], b[k] * p.decay);
       }
-      *(f32x4_t*)(p.w + o) = a;
-      *(f32x4_t*)(p.w + o + 4) = b;
+      *(f32x4_any*)(p.w + o) = a;
+      *(f32x4_any*)(p.w + o + 4) = b;
       if (p.copy) {
-        uint4 u;
+        u32x4_any u;
         u.x = f2bf(a[0]) | (uint32_t)f2bf(a[1]) << 16; u.y = f2bf(a[2]) | (uint32_t)f2bf(a[3]) << 16;
         u.z = f2bf(b[0]) | (uint32_t)f2bf(b[1]) << 16; u.w = f2bf(b[2]) | (uint32_t)f2bf(b[3]) << 16;
-        *(uint4*)(p.copy + o) = u;
+        *(u32x4_any*)(p.copy + o) = u;
       }
     }
     return;
@@ -300,10 +288,6 @@ __device__ __forceinline__ void ns_result8(const NsGemm& p, int z, int m, int n,
       if (p.copy) p.copy[o + r] = f2bf(w);
     }
   }
-}
-
-static void ns_set_vec(NsGemm& p) {
-  p.vec = p.Cc % 8 == 0 && (uintptr_t)p.C % 16 == 0 && (uintptr_t)p.w % 16 == 0 && (uintptr_t)p.copy % 16 == 0 && (uintptr_t)p.lo % 16 == 0;
 }
 
 // 256x256 tiles on the 8-phase loop (nt8.h): the three plane pairs as one run of 3 K / 64 K steps
@@ -1051,7 +1035,6 @@ static int ns_small_run(const MuonIn& in, NsGemm fin, int B, int steps, float ep
   NS_TRY(hipGetLastError());
   fin.R = in.R; fin.Cc = in.C; fin.il = in.il; fin.nb = in.B;
   fin.cs = 1.f / (float)(1L << (SP + SX));
-  ns_set_vec(fin);
   for (int k = 0; k < steps; ++k) {
     p.gin = w.g[k & 1];
     p.gout = w.g[~k & 1];
@@ -1139,7 +1122,6 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
       ap.B = b; ap.ldb = mp; ap.pb = tall ? w.ps : w.px; ap.bb = 2 * ap.pb;
       ap.M = Rp; ap.N = Cp; ap.K = mp; ap.cs = e2(-sq - SX);
       ap.R = in.R; ap.Cc = in.C; ap.il = in.il; ap.nb = in.B;
-      ns_set_vec(ap);
       NS_TRY(ns_launch<LAST>(ap, B, s));
     }
   }
