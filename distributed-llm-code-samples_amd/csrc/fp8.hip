@@ -21,7 +21,9 @@ typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 // columns sit in 16 neighbouring lanes (row scales: 4 rotations within them), a column's 128 rows in 16 values of g (column
 // scales: two lane exchanges that leave each of the wave's four g with two of the eight columns, then LDS over the four
 // waves).  x^T leaves through LDS so that its rows are written in whole 128-B lines; its rows there are 33 words apart, which
-// spreads both the writes and the reads over all banks.
+// spreads both the writes and the reads over all banks.  Bound by HBM on large tensors: 8192 x 4096 bf16, both orientations,
+// 28.6 us (4.7 TB/s; 42.8 with a row's load waited for before the next, exchanges through LDS and rows 36 words apart); a
+// tile takes about 5 us, which bounds small ones.
 // ----------------------------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f32(T v);
 template <> __device__ __forceinline__ float to_f32<uint16_t>(uint16_t v) { return bf2f(v); }
@@ -346,6 +348,10 @@ __device__ __forceinline__ void f8_epi1(const Fp8GemmArgs& p, int m, int n, floa
 // holds them, and 16 bits its two B rows; the matrix instruction picks the byte (op_sel), so scaling costs two 4-byte and
 // two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more: the last step again, with scale
 // bytes 0 on both sides, 2^-254 of it, which leaves every fp32 sum as it is.
+//
+// 8192 x 16384 x 4096 bf16: 444 us (2464 TF; 2898 in a library product without scales).  4096 x 16384 x 8192 fp32 with beta: 925
+// us (1190 TF; 1464 in a library bf16 product).  Bound by the matrix units' power, and at the tile boundary by every block
+// storing at once.
 // ----------------------------------------------------------------------------------------------
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));

@@ -221,6 +221,7 @@ struct NsGemm {
   void* C; int cdt, R, Cc;             // NS_OUT: result [R][Cc] (DT_BF16 / DT_F32);  NS_STEP: rows / columns of W
   int il, nb;                          // NS_STEP: alternating rows, as in MuonIn
   float* w; uint16_t* copy; int16_t* lo; float decay, rate;   // NS_STEP: fp32 master (+ bf16 copy), or split (lo, copy)
+  int ksplit; float* part;             // slices of K, each block's fp32 sums to part (ns_join adds them)
   int sym;                             // the product is symmetric: tiles on and below the diagonal, mirrored on writing
 };
 
@@ -468,6 +469,63 @@ template <int F> struct W4 {
   static constexpr int LDS = STAGES * STAGE;
 };
 
+// the tile's results from a lane's accumulators
+template <int EPI, int F>
+__device__ __forceinline__ void ns_w4_finish(const NsGemm& p, int z, int m0, int n0, int wid, int lane, const f32x4_t (&acc)[F][F]) {
+  const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
+  // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
+  constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
+  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
+  f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
+  const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
+  const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
+#pragma unroll
+  for (int c8 = 0; c8 < F / 2; ++c8) {            // 8 columns at a time
+    const int n = nb + 8 * c8;
+    if (n >= p.N) continue;
+    f16 th[8][F], tl[8][F];
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      const int m = mb + i;
+      if (m < p.M) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i][(8 * c8 + e) % F][(8 * c8 + e) / F];
+        if constexpr (PL) {
+          ns_value8<EPI>(p, z, m, n, v);
+          f16x8_t h, l;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f16 hh, ll;
+            split16(v[e], hh, ll);
+            h[e] = hh; l[e] = ll;
+            th[e][i] = hh; tl[e][i] = ll;
+          }
+          const long o = (long)z * p.bo + (long)m * p.ldo + n;
+          *(f16x8_t*)(p.out + o) = h;
+          *(f16x8_t*)(p.out + p.po + o) = l;
+        } else {
+          ns_result8<EPI>(p, z, m, n, v);
+        }
+      }
+    }
+    if (EPI == NS_PLANES_T || mirror) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f16* o = tp + (long)(n + e) * ldt + mb;
+#pragma unroll
+        for (int i = 0; i < F; i += 2) {          // rows are even and M is a multiple of 128: pairs are inside or outside
+          if (mb + i < p.M) {
+            typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+            *(f16x2_t*)(o + i) = f16x2_t{th[e][i], th[e][i + 1]};
+            *(f16x2_t*)(o + pt + i) = f16x2_t{tl[e][i], tl[e][i + 1]};
+          }
+        }
+      }
+    }
+  }
+}
+
 template <int EPI, int F>
 __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) {
   using W = W4<F>;
@@ -486,9 +544,10 @@ __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) 
     ao[i] = (uint32_t)((long)min(row, p.M - 1 - m0) * p.lda * 2 + c * 16);
     bo[i] = (uint32_t)((long)min(row, p.N - 1 - n0) * p.ldb * 2 + c * 16);
   }
-  const char* A = (const char*)(p.A + (long)z * p.ba + (long)m0 * p.lda);
-  const char* B = (const char*)(p.B + (long)z * p.bb + (long)n0 * p.ldb);
-  const int per = p.K >> 6, nk = 3 * per;
+  // slice blockIdx.y of the K steps (whole pairs of them)
+  const int k0 = (p.K >> 7) * blockIdx.y / p.ksplit * 2, per = (p.K >> 7) * (blockIdx.y + 1) / p.ksplit * 2 - k0, nk = 3 * per;
+  const char* A = (const char*)(p.A + (long)z * p.ba + (long)m0 * p.lda + (long)k0 * 64);
+  const char* B = (const char*)(p.B + (long)z * p.bb + (long)n0 * p.ldb + (long)k0 * 64);
   // next step to fetch: (hi, lo), (lo, hi), (hi, hi); past the last one it stays there
   const char *fa = A, *fb = B + p.pb * 2;
   int fleft = per, fseg = 0;
@@ -588,57 +647,31 @@ __device__ __forceinline__ void ns_w4_body(const NsGemm& p, DLLM_LDS char* lds) 
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-  // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
-  constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
-  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
-  f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
-  const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
-  const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
+  if constexpr (F == 2 && EPI == NS_PLANES) {
+    if (p.ksplit > 1) {
+      f32x4_t* o = (f32x4_t*)p.part + ((long)blockIdx.y * gridDim.x + blockIdx.x) * (F * F * 256) + t;
 #pragma unroll
-  for (int c8 = 0; c8 < F / 2; ++c8) {            // 8 columns at a time
-    const int n = nb + 8 * c8;
-    if (n >= p.N) continue;
-    f16 th[8][F], tl[8][F];
-#pragma unroll
-    for (int i = 0; i < F; ++i) {
-      const int m = mb + i;
-      if (m < p.M) {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[i][(8 * c8 + e) % F][(8 * c8 + e) / F];
-        if constexpr (PL) {
-          ns_value8<EPI>(p, z, m, n, v);
-          f16x8_t h, l;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f16 hh, ll;
-            split16(v[e], hh, ll);
-            h[e] = hh; l[e] = ll;
-            th[e][i] = hh; tl[e][i] = ll;
-          }
-          const long o = (long)z * p.bo + (long)m * p.ldo + n;
-          *(f16x8_t*)(p.out + o) = h;
-          *(f16x8_t*)(p.out + p.po + o) = l;
-        } else {
-          ns_result8<EPI>(p, z, m, n, v);
-        }
-      }
-    }
-    if (EPI == NS_PLANES_T || mirror) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f16* o = tp + (long)(n + e) * ldt + mb;
-#pragma unroll
-        for (int i = 0; i < F; i += 2) {          // rows are even and M is a multiple of 128: pairs are inside or outside
-          if (mb + i < p.M) {
-            typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
-            *(f16x2_t*)(o + i) = f16x2_t{th[e][i], th[e][i + 1]};
-            *(f16x2_t*)(o + pt + i) = f16x2_t{tl[e][i], tl[e][i + 1]};
-          }
-        }
-      }
+      for (int i = 0; i < F * F; ++i) o[i * 256] = acc[i / F][i % F];
+      return;
     }
   }
+  ns_w4_finish<EPI, F>(p, z, m0, n0, wid, lane, acc);
+}
+
+// slices of a product's K added up in order, and its results; grid as the product's, without the slices
+template <int EPI>
+__global__ __launch_bounds__(256) void ns_join(NsGemm p) {
+  const int t = threadIdx.x;
+  int z, m0, n0;
+  ns_tile<64>(p, z, m0, n0);
+  f32x4_t acc[2][2];
+  const f32x4_t* q = (const f32x4_t*)p.part + (long)blockIdx.x * 1024 + t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = q[i * 256];
+  for (int k = 1; k < p.ksplit; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] += q[(long)k * gridDim.x * 1024 + i * 256];
+  ns_w4_finish<EPI, 2>(p, z, m0, n0, t >> 6, t & 63, acc);
 }
 
 // 128 x 128: dynamic LDS (128 KiB, one block per CU) and a bound of two blocks, so that the compiler stays within 256
@@ -667,8 +700,27 @@ static int ns_cus() {
   return n;
 }
 
+// Slices of K for the Gram matrix of an m x n matrix (padded sizes): where its 64x64 tiles leave CUs empty and K is long, one
+// block's 3 n / 64 steps (0.24 us each) are shared by up to 16, for a launch that adds them up (6 us).  By the matrix's own
+// sizes, so that a batch gives the bits of the single matrix.  Orthogonalising 256 x 4096 to fp32: 268 ->
+// 157 us, 512 x 8192: 521 -> 321, 512 x 2048: 214 -> 173
+static int ns_slices(long m, long n) {
+  const long t = m / 64, tiles = t * (t + 1) / 2, per = n / 64;
+  int s = 1;
+  while (s < 16 && tiles * (2 * s) <= 256 && per >= 8 * (2 * s)) s *= 2;
+  return s > 1 && 3.f * (float)per * 0.24f * (1.f - 1.f / (float)s) > 6.f ? s : 1;
+}
+
 template <int EPI>
-static hipError_t ns_launch(const NsGemm& p, int B, hipStream_t s) {
+static hipError_t ns_launch(NsGemm p, int B, hipStream_t s) {
+  if (EPI == NS_PLANES && p.ksplit > 1) {
+    const long grid = (long)B * ns_tiles(p, 64);
+    if (grid > 0x7fffffffL) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((ns_gemm_64<NS_PLANES>), dim3((unsigned)grid, p.ksplit), dim3(256), 0, s, p);
+    hipLaunchKernelGGL((ns_join<NS_PLANES>), dim3((unsigned)grid), dim3(256), 0, s, p);
+    return hipGetLastError();
+  }
+  p.ksplit = 1;
   // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU (measured on full
   // rounds: 128 x 128 is bound by LDS, the larger ones by the matrix units' power), and of a round's beginning and end
   const long cus = ns_cus();
@@ -703,6 +755,8 @@ struct NsSpace {
   long px, ps;              // elements of an X (or X^T) and of an m x m plane
   double* part;
   f16 *X, *XT, *XT2, *S[6];
+  int slices;               // of the Gram matrix's K, and their sums
+  float* sums;
   size_t bytes;
 };
 static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
@@ -722,6 +776,9 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
   w.XT = (f16*)take((size_t)B * w.px * 4);
   w.XT2 = again ? (f16*)take((size_t)B * w.px * 4) : nullptr;
   for (int i = 0; i < 6; ++i) w.S[i] = (f16*)take((size_t)B * w.ps * 4);
+  w.slices = ns_slices(w.mp, w.np);
+  const long t = w.mp / 64;
+  w.sums = w.slices > 1 ? (float*)take((size_t)B * w.slices * (t * (t + 1) / 2) * 4096 * 4) : nullptr;
   w.bytes = o;
   return w;
 }
@@ -738,7 +795,7 @@ static NsSpace ns_space(char* base, int B, int R, int C, bool again) {
 // A and P (128 x 128, padded with zeros) fit a block, so every block computes P for itself and applies it to its own columns
 // of X, then leaves its part of the next A, the fp32 Gram matrix of the columns it just wrote; the next launch adds the
 // parts up in their order.  Launches and their latency bound it: 300 x 101, five steps, 17 launches of the kernels above
-// take 87 us.
+// take 87 us, these 7 take 70; 16 x 16 87 and 48.
 //
 // X lives in operand order, "fragments": chunk (nt, kk) of a plane is 64 lanes x 8 values, lane (g, i) = (lane / 16,
 // lane % 16) holding column 16 nt + i, rows 32 kk + 4 g + (0 .. 3) and 32 kk + 16 + 4 g + (0 .. 3).  That is what a lane has
@@ -884,7 +941,7 @@ __global__ __launch_bounds__(256) void ns_small_sum(const float* in, int parts, 
 
 // one step.  EPI NS_PLANES: X <- P X in place, and its parts of the next A; NS_OUT / NS_STEP: the result.  Sixteen waves of
 // little code: every instruction is fetched once per launch, at about 0.7 us a kilobyte, and four waves with four times the
-// code each took 14 to 18 us a launch
+// code each took 14 to 18 us a launch (these: 6 for 16 x 16, 12 for 300 x 101, of which LDS reads and matrix instructions are 7)
 template <int EPI>
 __global__ __launch_bounds__(1024) void ns_small_step(NsSmall p, NsGemm fin) {
   __shared__ __attribute__((aligned(16))) f16x8_t af[2 * 32 * 64];   // A's fragments, then P's: chunk kk * 8 + mt
@@ -1087,6 +1144,7 @@ static int ns_run(const MuonIn& in, NsGemm fin, int B, int steps, int seg, float
     left -= n;
     NsGemm gr = square(w.X, w.X, A, e2(SA - 2 * SX));
     gr.lda = gr.ldb = np; gr.pa = gr.pb = w.px; gr.ba = gr.bb = 2 * w.px; gr.K = np;
+    gr.ksplit = w.slices; gr.part = w.sums;
     NS_TRY(ns_launch<NS_PLANES>(gr, B, s));
     int sq = SP;
     for (int i = 0; i < n; ++i) {

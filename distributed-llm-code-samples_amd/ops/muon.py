@@ -172,7 +172,7 @@ def muon_step_(master: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor,
     ``momentum = beta·momentum + g``, ``U = g + beta·momentum`` (``nesterov``) or ``momentum``, ``O = orthogonalize(U)``,
     ``master = (1 - lr·wd)·master - lr·scale·O``, ``copy = bf16(master)``,  with ``g = grad_scale·grad`` (bf16 or fp32).
     ``scale`` defaults to ``muon_scale(R, C)``.  ``interleave``: ``master`` [2 R, C] holds two matrices whose rows alternate
-    in blocks of that many (the gated FFN's W13), each stepped as its own."""
+    in blocks of that many (the gated FFN's W13), each stepped as its own.  No two of the tensors may share memory."""
     if master.dtype != torch.float32:
         raise TypeError("master weights must be fp32")
     _step(grad, momentum, lr, beta, nesterov, wd, steps, eps, scale, grad_scale, interleave, master, copy, None)

@@ -87,7 +87,7 @@ def test_muon_engine_masters_agree(fp8, gated, master):
 
 def test_muon_interleaved_equals_separate():
     g = torch.Generator().manual_seed(5)
-    for R, C, il in ((512, 96, 16), (96, 200, 1), (640, 256, 64)):
+    for R, C, il in ((512, 96, 16), (96, 200, 1), (64, 9, 1), (900, 301, 3), (640, 256, 64)):
         w, gr, m = (torch.randn(R, C, generator=g).to(DEV) for _ in range(3))
         pick = lambda t, i: t.view(-1, 2, il, C)[:, i].reshape(-1, C).contiguous()  # noqa: E731
         parts = [[pick(t, i) for t in (w, gr, m)] for i in range(2)]
@@ -136,6 +136,24 @@ def test_step_captured_and_replayed():
                 assert torch.equal(eager[part][k], graphed[part][k]), (part, k)
         assert torch.equal(eager["y"], graphed["y"])
         x.copy_(torch.randn(T, D, device=DEV))
+
+
+@pytest.mark.parametrize("kw", [{"optimizer": "muon"}, {"fp8": True}, {"optimizer": "muon", "fp8": True}])
+def test_side_stream_optimizer_agrees(kw):
+    """The update on the side stream (side_optimizer -1) equals the update in order, over steps that reuse the buffers."""
+    layers = _layers(128, 256, 3)
+    res = []
+    for side in (0, -1):
+        cfg = TrainConfig(model=ModelConfig(128, 256, 3), batch_size=1, seq_len=64, lr=0.01, dtype="bf16", side_optimizer=side,
+                          grad_dtype="fp32", **kw)
+        eng = FFNTrainer(cfg, Mesh(), torch.device(DEV))
+        eng.load_full_params(layers)
+        for seed in range(3):
+            eng.train_step(*_data(64, 128, seed))
+        torch.cuda.synchronize()
+        res.append(eng.gather_full_params())
+    for a, b in zip(*res):
+        assert all(torch.equal(a[k], b[k]) for k in a)
 
 
 def test_graphed_step_refuses():

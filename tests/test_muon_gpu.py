@@ -72,6 +72,14 @@ def test_batch_is_bitwise_the_single_matrix():
     assert torch.equal(out, muon.orthogonalize(x))
 
 
+@pytest.mark.parametrize("R,C", [(200, 3000), (400, 2100)])
+def test_batch_of_sliced_grams_is_bitwise_the_single_matrix(R, C):
+    x = gradient(R, C, 4, batch=3).to(DEV)
+    got = muon.orthogonalize(x)
+    for i in range(3):
+        assert torch.equal(got[i], muon.orthogonalize(x[i]))
+
+
 def test_magnitudes_and_non_finite():
     """The result does not depend on the update's magnitude until eps = 1e-7 counts; zero stays zero; NaN and inf spoil their
     own matrix of a batch and no other."""
@@ -158,7 +166,8 @@ def test_other_stream_and_graph():
         assert torch.equal(w, we) and torch.equal(m, me)
 
 
-@pytest.mark.parametrize("R,C", [(4096, 4224), (8192, 4096), (2900, 3100), (1024, 8200), (2048, 2048), (1300, 1300)])
+@pytest.mark.parametrize("R,C", [(4096, 4224), (8192, 4096), (2900, 3100), (1024, 8200), (2048, 2048), (1300, 1300), (200, 5000),
+                                 (5000, 260), (511, 2050), (150, 30000)])
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
 def test_orthogonalize_large(R, C, out):
     """Sizes that take the larger tiles, against the iteration in 64 bits; memory that the workspace may get holds NaN."""
