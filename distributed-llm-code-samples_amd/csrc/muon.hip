@@ -375,19 +375,33 @@ static __host__ __device__ inline int ns_tiles(const NsGemm& p, int ts) {
   return p.sym ? a * (a + 1) / 2 : a * b;
 }
 
+// A symmetric product's elements above the diagonal, and whether the lane's rows from m and columns from n are written as
+// they are (0), also mirrored (1), or left to the mirror (-1).  Above and below the diagonal the same number is rounded
+// differently: the plane pairs are added in exchanged order, and (P A) P is symmetric only up to rounding.  So which of the
+// two is taken goes by 64x64 blocks, whatever the tile: on the diagonal each its own, elsewhere the lower one.  The tile depends on
+// the batch (ns_launch), a matrix's bits do not.  (Tiles are multiples of 64, no lane's rows or columns cross that border
+// but those of 192x192 tiles, which ask row by row.)
+template <int EPI>
+__device__ __forceinline__ int ns_half(const NsGemm& p, int m, int n) {
+  if (EPI != NS_PLANES && EPI != NS_POLY) return 0;
+  if (!p.sym) return 0;
+  const int d = (m >> 6) - (n >> 6);
+  return d > 0 ? 1 : d < 0 ? -1 : 0;
+}
+
 // the tile's results from its accumulators
 template <int EPI>
 __device__ __forceinline__ void ns_finish(const NsGemm& p, int z, int m0, int n0, int wid, int lane,
                                           const f32x4_t (&acc)[2][2][4][2]) {
   constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
-  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
   f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
   const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
 #pragma unroll
   for (int qm = 0; qm < 2; ++qm)
 #pragma unroll
     for (int qn = 0; qn < 2; ++qn) {
-      const int n = n0 + n8_col(wid, lane, qn);
+      const int n = n0 + n8_col(wid, lane, qn), half = ns_half<EPI>(p, m0 + n8_row(wid, lane, qm, 0), n);
+      if (half < 0) continue;
       f16x4_t th[8], tl[8];   // transposed planes: column n + e, rows of the four mt
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -414,7 +428,7 @@ __device__ __forceinline__ void ns_finish(const NsGemm& p, int z, int m0, int n0
           ns_result8<EPI>(p, z, m, n, v);
         }
       }
-      if (EPI == NS_PLANES_T || mirror) {
+      if (EPI == NS_PLANES_T || half > 0) {
         const int m = m0 + n8_row(wid, lane, qm, 0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -475,7 +489,6 @@ __device__ __forceinline__ void ns_w4_finish(const NsGemm& p, int z, int m0, int
   const int i15 = lane & 15, g = lane >> 4, wr = wid >> 1, wc = wid & 1;
   // lane: rows mb .. mb + F - 1, columns nb .. nb + 4F - 1 (column F r + k of them: acc[.][k][r])
   constexpr bool PL = EPI == NS_PLANES || EPI == NS_PLANES_T || EPI == NS_POLY;
-  const bool mirror = PL && EPI != NS_PLANES_T && p.sym && m0 != n0;
   f16* tp = EPI == NS_PLANES_T ? p.outT + (long)z * p.bt : p.out + (long)z * p.bo;
   const long ldt = EPI == NS_PLANES_T ? p.ldt : p.ldo, pt = EPI == NS_PLANES_T ? p.pt : p.po;
   const int mb = m0 + wr * 16 * F + F * i15, nb = n0 + wc * 16 * F + 4 * F * g;
@@ -487,7 +500,7 @@ __device__ __forceinline__ void ns_w4_finish(const NsGemm& p, int z, int m0, int
 #pragma unroll
     for (int i = 0; i < F; ++i) {
       const int m = mb + i;
-      if (m < p.M) {
+      if (m < p.M && ns_half<EPI>(p, m, n) >= 0) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = acc[i][(8 * c8 + e) % F][(8 * c8 + e) / F];
@@ -509,13 +522,13 @@ __device__ __forceinline__ void ns_w4_finish(const NsGemm& p, int z, int m0, int
         }
       }
     }
-    if (EPI == NS_PLANES_T || mirror) {
+    if (EPI == NS_PLANES_T || ns_half<EPI>(p, mb + F - 1, n) > 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         f16* o = tp + (long)(n + e) * ldt + mb;
 #pragma unroll
-        for (int i = 0; i < F; i += 2) {          // rows are even and M is a multiple of 128: pairs are inside or outside
-          if (mb + i < p.M) {
+        for (int i = 0; i < F; i += 2) {          // rows are even, M a multiple of 128: pairs are on one side of its end
+          if (mb + i < p.M && (EPI == NS_PLANES_T || ns_half<EPI>(p, mb + i, n) > 0)) {   // (and of a 64x64 block's)
             typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
             *(f16x2_t*)(o + i) = f16x2_t{th[e][i], th[e][i + 1]};
             *(f16x2_t*)(o + pt + i) = f16x2_t{tl[e][i], tl[e][i + 1]};
