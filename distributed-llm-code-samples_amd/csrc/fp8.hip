@@ -346,8 +346,10 @@ __device__ __forceinline__ void f8_epi1(const Fp8GemmArgs& p, int m, int n, floa
 //
 // Scales: a lane's four A rows of a half are consecutive rows of C (nt8.h), so one 32-bit word of the K step's scale row
 // holds them, and 16 bits its two B rows; the matrix instruction picks the byte (op_sel), so scaling costs two 4-byte and
-// two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more: the last step again, with scale
-// bytes 0 on both sides, 2^-254 of it, which leaves every fp32 sum as it is.
+// two 2-byte loads per K step and nothing else.  An odd number of K steps runs one more, the last step again, without effect: a
+// bf16 result takes it with scale bytes 0 on both sides, 2^-254 of products whose infinities stay infinities, which leaves
+// every sum as it is (jumping over its matrix instructions costs that kernel 270 bytes of spills); an fp32 result jumps over
+// them, as codes times 2^-127 would be rounded to zero in bf16, and infinity times zero is NaN.
 //
 // 8192 x 16384 x 4096 bf16: 444 us (2464 TF; 2898 in a library product without scales).  4096 x 16384 x 8192 fp32 with beta: 925
 // us (1190 TF; 1464 in a library bf16 product).  Bound by the matrix units' power, and at the tile boundary by every block
@@ -413,12 +415,15 @@ struct F8Trait {
   }
   template <int QM, int QN, int ODD>
   __device__ __forceinline__ void mma(f32x4_t (&c)[4][2], N8Frag (&fa)[4], N8Frag (&fb)[2]) {
+    if constexpr (ODD && EXACT) {
+      if (keep == 0) return;
+    }
     if constexpr (QM == 0 && QN == 0) {   // the step's first phase
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         wa[ODD][h] = (int)((uint32_t)wa[ODD][h] >> (sh >> (8 * h) & 31));
         wb[ODD][h] = (int)((uint32_t)wb[ODD][h] >> (sh >> (16 + 8 * h) & 31));
-        if constexpr (ODD) { wa[ODD][h] &= keep; wb[ODD][h] &= keep; }
+        if constexpr (ODD && !EXACT) { wa[ODD][h] &= keep; wb[ODD][h] &= keep; }
       }
     }
     const int a = wa[ODD][QM], b = wb[ODD][QN];
