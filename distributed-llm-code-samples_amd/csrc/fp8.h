@@ -11,7 +11,6 @@
 namespace dllm {
 
 enum Fp8Fmt : int { F8_E4M3 = 0, F8_E5M2 = 1 };   // also the matrix instruction's operand format codes
-constexpr int F8_BLOCK = 128;
 
 // 2^(b - 127) of an exponent byte (b = 255: NaN, b = 0: the subnormal 2^-127)
 __device__ __forceinline__ float e8m0_to_f32(uint32_t b) {

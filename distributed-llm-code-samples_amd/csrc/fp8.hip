@@ -7,7 +7,6 @@
 namespace dllm {
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
-typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(2))) float f32x2_t;
 
 // 16-byte accesses at any element's address: the hardware takes them unaligned, so odd row lengths need no other path
@@ -292,11 +291,6 @@ __global__ __launch_bounds__(256) void fp8_dequantize_kernel(const uint8_t* q, l
 // consecutive columns of a row of C.  Three kernels: 256x256 tiles (8-phase loop), 128x128 and 64x64 tiles (one wave per
 // quarter), and few rows or columns (operands straight to registers, K over the waves); fp8_plan picks.
 // ----------------------------------------------------------------------------------------------
-template <int FB, int FA>
-__device__ __forceinline__ f32x4_t mfma_f8(i32x8_t b, i32x8_t a, f32x4_t c, int sb, int sa) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, c, FB, FA, 0, sb, 0, sa);
-}
-
 // The 8-bit matrix instruction adds the products of 8 neighbouring k with 13 bits below the largest of them (measured: a
 // product under 2^-13 of its neighbour is lost whole, the sums of 8 then add up in fp32): about 4e-5 of the result, a
 // hundredth of bf16's half step 2^-8 but hundreds of fp32's.  So a bf16 result is computed on it, and an fp32 result on
@@ -857,15 +851,6 @@ __global__ __launch_bounds__(512) void fp8_gemm_rows(Fp8GemmArgs p) {
 // ----------------------------------------------------------------------------------------------
 // choice and launch
 // ----------------------------------------------------------------------------------------------
-static int fp8_cus() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
-    return v;
-  }();
-  return n;
-}
-
 template <int EPI, typename OutT, int FA, int FB>
 static hipError_t launch_fp8_f(Fp8GemmArgs p, hipStream_t s) {
   const int few = min(p.M, p.N);
@@ -920,7 +905,7 @@ static void fp8_plan(int M, int N, int nk, bool exact, int& tile, int& ksplit) {
   float best = 1e30f;
   tile = 128;
   ksplit = 1;
-  const long cus = fp8_cus();
+  const long cus = cu_count();
   const int few = (min(M, N) + 15) / 16 * 16;
   if (few <= FP8_FEW) {
     // a block reads its 16 long rows and all of the short operand, at about 30 KB/us on a CU

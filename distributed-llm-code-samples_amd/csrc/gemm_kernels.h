@@ -2231,7 +2231,8 @@ constexpr bool persistent_kernel();
 template <int L, int E, typename OutT, int ACT>
 static void launch_pp_act(const GemmArgs& a0, hipStream_t s) {
   const int nb0 = (a0.M / BT_M) * (a0.N / PP_BN) * a0.ksplit;
-  // the persistent TN store into fp32 does not fit the register budget without packed fp32 math (256 B of scratch)
+  // the TN store into fp32 runs one tile per block: persistent, it does not fit the register budget without packed fp32 math
+  // (256 B of scratch), and made to fit it is slower (4096 x 16384 x 8192: 1019 us against 968; 16384 x 4096 x 8192: 938, 887)
   constexpr bool spills = L == L_TN && E == EPI_STORE && std::is_same<OutT, float>::value;
   if constexpr (persistent_kernel<L, E, OutT, ACT>() && !spills) {
     GemmArgs a = a0;

@@ -704,15 +704,6 @@ __global__ __launch_bounds__(256, 1) void ns_gemm_192(NsGemm p) {
   ns_w4_body<EPI, 6>(p, (DLLM_LDS char*)smem);
 }
 
-static int ns_cus() {
-  static const int n = [] {
-    int dev = 0, v = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
-    return v;
-  }();
-  return n;
-}
-
 // Slices of K for the Gram matrix of an m x n matrix (padded sizes): where its 64x64 tiles leave CUs empty and K is long, one
 // block's 3 n / 64 steps (0.24 us each) are shared by up to 16, for a launch that adds them up (6 us).  By the matrix's own
 // sizes, so that a batch gives the bits of the single matrix.  Orthogonalising 256 x 4096 to fp32: 268 ->
@@ -736,7 +727,7 @@ static hipError_t ns_launch(NsGemm p, int B, hipStream_t s) {
   p.ksplit = 1;
   // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU (measured on full
   // rounds: 128 x 128 is bound by LDS, the larger ones by the matrix units' power), and of a round's beginning and end
-  const long cus = ns_cus();
+  const long cus = cu_count();
   const float steps = 3.f * (float)(p.K >> 6);
   auto time = [&](int ts, long per_cu, float step) {
     return (float)(((long)B * ns_tiles(p, ts) + cus * per_cu - 1) / (cus * per_cu)) * (steps * step + 5.f);

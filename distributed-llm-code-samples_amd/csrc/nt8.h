@@ -32,7 +32,6 @@ constexpr int N8_HT = 16384;               // half-tile bytes
 constexpr int N8_LDS = 8 * N8_HT;
 
 typedef __attribute__((ext_vector_type(4))) int n8_i32x4;
-typedef __attribute__((ext_vector_type(8))) int n8_i32x8;
 
 #define N8_BARRIER()               \
   do {                             \
@@ -57,6 +56,16 @@ __device__ __forceinline__ void n8_read(n8_i32x4& d, uint32_t addr) {
 __device__ __forceinline__ void n8_dma(const char* src, uint32_t off, DLLM_LDS char* dst) {
   __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)src, 0, 0x7fffffff, 0x00027000);
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (DLLM_LDS void*)dst, 16, (int)off, 0, 0, 0);
+}
+
+// CUs of the device (256 where there is none: plans are made on the host)
+static inline int cu_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || v <= 0) v = 256;
+    return v;
+  }();
+  return n;
 }
 
 // dynamic LDS beyond 64 KiB is allowed per kernel, once
