@@ -23,7 +23,7 @@ _ERR: str | None = None
 c_int, c_long, c_float, c_void_p, c_ull = ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_void_p, ctypes.c_ulonglong
 
 # bumped with every signature or stream-semantics change below (csrc/elementwise.hip dllm_abi_version): a stale library fails loudly
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _SIGS = {
     "dllm_gemm": (c_int, [c_int, c_int, c_int, c_int, c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_long,
@@ -61,9 +61,9 @@ _SIGS = {
     "dllm_fp8_gemm": (c_int, [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_long, c_void_p, c_long, c_int,
                               c_void_p, c_long, c_int, c_void_p, c_void_p, c_long, c_int, c_int, c_int, c_float, c_float,
                               c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
-    "dllm_fp8_gemm_plan": (c_int, [c_int, c_int, c_int, c_int]),
+    "dllm_fp8_gemm_plan": (c_int, [c_int, c_int, c_int, c_int, c_long]),
     "dllm_linear_fp8_workspace": (c_long, [c_int, c_int, c_int, c_int]),
-    "dllm_linear_fp8_bwd_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
+    "dllm_linear_fp8_bwd_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int, c_long, c_long]),
     "dllm_linear_fp8": (c_int, [c_void_p, c_int, c_long, c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_void_p,
                                 c_void_p, c_void_p, c_void_p, c_int, c_long, c_void_p, c_long, c_void_p]),
     "dllm_linear_fp8_bwd": (c_int, [c_void_p, c_int, c_long, c_int, c_int, c_int, c_void_p, c_long, c_void_p, c_long, c_int,

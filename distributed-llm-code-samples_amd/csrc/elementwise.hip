@@ -671,6 +671,6 @@ int dllm_queue_reserve(void* base, int candidates, int spin_us) {
   return err ? err : nblock;
 }
 
-int dllm_abi_version() { return 15; }
+int dllm_abi_version() { return 16; }
 
 }  // extern "C"

@@ -895,6 +895,10 @@ static hipError_t launch_fp8(const Fp8GemmArgs& p, int fa, int fb, hipStream_t s
 }
 
 constexpr int FP8_FEW = 64;   // rows (or columns) that fp8_gemm_rows takes, at most
+// its blocks of 512 threads count 16 long rows each, and a launch counts its threads in 32 bits
+constexpr int FP8_LONG = (1 << 27) - 16;
+// bytes from row to row that the tiles' fetches take: the buffer form reaches 2^31 bytes from a tile's first row
+constexpr long FP8_PITCH = (0x7fffffffL - 4096) / 256;
 
 // Tile (0: fp8_gemm_rows) and number of K slices: the least time for whole rounds of CUs, in microseconds measured on full
 // rounds: a K step of 128 on one CU (bf16 results / fp32 results), a round's beginning and end, and the slices' partial sums
@@ -965,11 +969,19 @@ int dllm_fp8_dequantize(const void* q, long ldq, const void* sq, long ldsq, int 
   return (int)hipGetLastError();
 }
 
-// tile size (low 16 bits) and K slices (high 16) that dllm_fp8_gemm should be given; ksplit > 1 needs ksplit * M * N floats
-int dllm_fp8_gemm_plan(int M, int N, int nk, int out_dtype) {
+// tile size (low 16 bits) and K slices (high 16) that dllm_fp8_gemm should be given; ksplit > 1 needs ksplit * M * N floats.
+// `pitch`: the larger of the operands' row strides.  -1 for sizes that no kernel takes: a pitch above FP8_PITCH with more than
+// FP8_FEW rows on both sides, more than FP8_LONG rows next to few
+int dllm_fp8_gemm_plan(int M, int N, int nk, int out_dtype, long pitch) {
   int tile, ksplit;
   fp8_plan(M, N, nk, out_dtype == DT_F32, tile, ksplit);
   if (nk == 0 && tile == 256) tile = 128;
+  if (tile != 0 && nk > 0 && pitch > FP8_PITCH) {
+    if (min(M, N) > FP8_FEW) return -1;
+    tile = 0;
+    ksplit = 1;
+  }
+  if (tile == 0 && max(M, N) > FP8_LONG) return -1;
   return tile | ksplit << 16;
 }
 
@@ -990,12 +1002,12 @@ int dllm_fp8_gemm(const void* A, long lda, const void* SA, long ldsa, int fa, co
   Fp8GemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)SA, ldsa, (const uint8_t*)B, ldb, (const uint8_t*)SB, ldsb,
                 C, ldc, aux, aux_out, ldaux, M, N, nk, alpha, beta, act, tile, ksplit, ws};
   if (tile == 0) {
-    if (min(M, N) > FP8_FEW || ksplit != 1) return -1;
+    if (min(M, N) > FP8_FEW || max(M, N) > FP8_LONG || ksplit != 1) return -1;
   } else {
-    // the buffer-form fetches reach 2^31 bytes from a tile's first row; scale words span 4 (2) rows, which these have
+    // scale words span 4 (2) rows, which these have
     if (min(M, N) <= 16 || (tile != 64 && tile != 128 && tile != 256) || ksplit < 1 || ksplit > 8 || (ksplit > 1 && (ws == nullptr || tile == 256)))
       return -1;
-    if (max(lda, ldb) > (0x7fffffffL - 4096) / 256 || (nk == 0 && tile == 256)) return -1;
+    if ((nk > 0 && max(lda, ldb) > FP8_PITCH) || (nk == 0 && tile == 256)) return -1;
   }
   hipStream_t s = (hipStream_t)stream;
   const bool bf = out_dtype == DT_BF16;
@@ -1027,32 +1039,38 @@ static LinWs lin_ws(char* base, long ra, long ka, long rb, long kb, long part) {
   w.bytes = o;
   return w;
 }
-// floats that a product's K slices need
-static long lin_part(int M, int N, int K, int odt) {
-  const int t = dllm_fp8_gemm_plan(M, N, (K + 127) / 128, odt) >> 16;
+// floats that a product's K slices need; operands in rows of `pitch` bytes
+static long lin_part(int M, int N, int K, int odt, long pitch) {
+  const int t = dllm_fp8_gemm_plan(M, N, (K + 127) / 128, odt, pitch) >> 16;
   return t > 1 ? (long)t * M * N : 0;
 }
+static long pad_k(int k) { return ((long)k + 127) / 128 * 128; }
 static int lin_gemm(const uint8_t* A, long lda, const uint8_t* SA, long ldsa, int fa, const uint8_t* B, long ldb,
                     const uint8_t* SB, long ldsb, int fb, void* C, long ldc, int odt, int M, int N, int K, float beta, float* part,
                     void* stream) {
-  const int nk = (K + 127) / 128, t = dllm_fp8_gemm_plan(M, N, nk, odt);
+  const int nk = (K + 127) / 128, t = dllm_fp8_gemm_plan(M, N, nk, odt, max(lda, ldb));
+  if (t < 0) return -1;
   return dllm_fp8_gemm(A, lda, SA, ldsa, fa, B, ldb, SB, ldsb, fb, C, ldc, odt, nullptr, nullptr, 0, M, N, nk, 1.f, beta, EPI_STORE,
                        ACT_NONE, t & 0xffff, t >> 16, part, stream);
 }
 
-// bytes of workspace of dllm_linear_fp8 (y of type odt) and of dllm_linear_fp8_bwd (dx, dw of types dxdt, dwdt)
-long dllm_linear_fp8_workspace(int T, int D, int F, int odt) { return lin_ws(nullptr, T, D, F, D, lin_part(T, F, D, odt)).bytes; }
-long dllm_linear_fp8_bwd_workspace(int T, int D, int F, int dxdt, int dwdt) {
-  return lin_ws(nullptr, T, F, F, T, max(lin_part(T, D, F, dxdt), lin_part(F, D, T, dwdt))).bytes;
+// bytes of workspace of dllm_linear_fp8 (y of type odt) and of dllm_linear_fp8_bwd (dx, dw of types dxdt, dwdt; wt and xt in rows
+// of ldwt and ldxt bytes)
+long dllm_linear_fp8_workspace(int T, int D, int F, int odt) { return lin_ws(nullptr, T, D, F, D, lin_part(T, F, D, odt, pad_k(D))).bytes; }
+static LinWs lin_bwd_ws(char* base, int T, int D, int F, int dxdt, int dwdt, long ldwt, long ldxt) {
+  return lin_ws(base, T, F, F, T, max(lin_part(T, D, F, dxdt, max(pad_k(F), ldwt)), lin_part(F, D, T, dwdt, max(pad_k(T), ldxt))));
+}
+long dllm_linear_fp8_bwd_workspace(int T, int D, int F, int dxdt, int dwdt, long ldwt, long ldxt) {
+  return lin_bwd_ws(nullptr, T, D, F, dxdt, dwdt, ldwt, ldxt).bytes;
 }
 
 // y [T, F] = x [T, D] w [F, D]^T; leaves x^T [D, T] and w^T [D, F] in 8 bits (rows of pad128 codes, dense scales)
 int dllm_linear_fp8(const void* x, int xdt, long ldx, const void* w, int wdt, long ldw, int T, int D, int F, void* xt, void* sxt,
                     void* wt, void* swt, void* y, int odt, long ldy, void* ws, long ws_bytes, void* stream) {
   if (T <= 0 || D <= 0 || F <= 0 || (odt != DT_BF16 && odt != DT_F32)) return -1;
-  const LinWs l = lin_ws((char*)ws, T, D, F, D, lin_part(T, F, D, odt));
+  const LinWs l = lin_ws((char*)ws, T, D, F, D, lin_part(T, F, D, odt, pad_k(D)));
   if (ws == nullptr || (uintptr_t)ws % 256 || ws_bytes < l.bytes) return -1;
-  const long pd = ((long)D + 127) / 128 * 128, pt = ((long)T + 127) / 128 * 128, pf = ((long)F + 127) / 128 * 128;
+  const long pd = pad_k(D), pt = pad_k(T), pf = pad_k(F);
   int rc = dllm_fp8_quantize(x, xdt, ldx, T, D, l.a, pd, l.sa, T, xt, pt, sxt, D, F8_E4M3, F8_E4M3, 0, stream);
   if (rc == 0) rc = dllm_fp8_quantize(w, wdt, ldw, F, D, l.b, pd, l.sb, F, wt, pf, swt, D, F8_E4M3, F8_E4M3, 1, stream);
   if (rc == 0) rc = lin_gemm(l.a, pd, l.sa, T, F8_E4M3, l.b, pd, l.sb, F, F8_E4M3, y, ldy, odt, T, F, D, 0.f, l.part, stream);
@@ -1064,9 +1082,9 @@ int dllm_linear_fp8_bwd(const void* dy, int ydt, long ldy, int T, int D, int F, 
                         long ldsxt, int fx, const void* wt, long ldwt, const void* swt, long ldswt, int fw, void* dx, int dxdt,
                         long lddx, void* dw, int dwdt, long lddw, float beta, void* ws, long ws_bytes, void* stream) {
   if (T <= 0 || D <= 0 || F <= 0 || (dwdt != DT_BF16 && dwdt != DT_F32) || (dxdt != DT_BF16 && dxdt != DT_F32)) return -1;
-  const LinWs l = lin_ws((char*)ws, T, F, F, T, max(lin_part(T, D, F, dxdt), lin_part(F, D, T, dwdt)));
+  const LinWs l = lin_bwd_ws((char*)ws, T, D, F, dxdt, dwdt, ldwt, ldxt);
   if (ws == nullptr || (uintptr_t)ws % 256 || ws_bytes < l.bytes || dw == nullptr) return -1;
-  const long pt = ((long)T + 127) / 128 * 128, pf = ((long)F + 127) / 128 * 128;
+  const long pt = pad_k(T), pf = pad_k(F);
   int rc = dllm_fp8_quantize(dy, ydt, ldy, T, F, dx ? l.a : nullptr, pf, dx ? l.sa : nullptr, T, l.b, pt, l.sb, F, F8_E5M2, F8_E5M2, 0,
                              stream);
   if (rc == 0 && dx)

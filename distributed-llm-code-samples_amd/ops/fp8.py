@@ -237,11 +237,24 @@ def _check_rows(t: torch.Tensor, name: str, shape: tuple, device) -> None:
         raise ValueError(f"{name} must be a row-major view without overlapping rows, got strides {t.stride()}")
 
 
+MAX_PITCH = (2 ** 31 - 1 - 4096) // 256    # bytes between rows that the tiled kernels take; the one for few rows takes any
+
+
 @functools.lru_cache(maxsize=4096)
-def _plan(M: int, N: int, kb: int, out_code: int) -> tuple[int, int]:
-    """(output tile, or 0 for the kernel for few rows, K slices) of a product's sizes and result type."""
-    p = _native.lib().dllm_fp8_gemm_plan(M, N, kb, out_code)
+def _plan(M: int, N: int, kb: int, out_code: int, pitch: int = 0) -> tuple[int, int]:
+    """(output tile, or 0 for the kernel for few rows, K slices) of a product's sizes and result type.  ``pitch``: the larger
+    row stride of the operands where it is above ``MAX_PITCH``."""
+    p = _native.lib().dllm_fp8_gemm_plan(M, N, kb, out_code, pitch)
+    if p < 0:
+        raise ValueError(f"8-bit product of {M} x {N}: with more than 64 rows on both sides operand rows are up to {MAX_PITCH} "
+                         f"bytes apart{f', got {pitch}' if pitch else ''}; with fewer, up to {2 ** 27 - 16} rows on the other side")
     return p & 0xFFFF, p >> 16
+
+
+def _far(*pitches: int) -> int:
+    """The largest row stride where it changes the choice of a kernel, else 0 (one cached plan for all others)."""
+    p = max(pitches)
+    return p if p > MAX_PITCH else 0
 
 
 def gemm_fp8(a: BlockFP8, b: BlockFP8, out: torch.Tensor | None = None, *, out_dtype: torch.dtype = torch.bfloat16,
@@ -285,7 +298,7 @@ def gemm_fp8(a: BlockFP8, b: BlockFP8, out: torch.Tensor | None = None, *, out_d
     if not ad.is_cuda:
         return _gemm_torch(a, b, out, alpha, beta, epi, act, aux, aux_out)
     nk = ad.shape[1] // BLOCK
-    tile, ksplit = _plan(M, N, nk, oc)
+    tile, ksplit = _plan(M, N, nk, oc, _far(aarg[1], barg[1]))
     ws = torch.empty(ksplit * M * N, dtype=torch.float32, device=dev) if ksplit > 1 else None
     with _on(dev):
         rc = _native.lib().dllm_fp8_gemm(
@@ -340,9 +353,17 @@ class LinearFP8(NamedTuple):
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_workspace(T: int, D: int, F: int, *codes: int) -> int:
-    f = _native.lib().dllm_linear_fp8_workspace if len(codes) == 1 else _native.lib().dllm_linear_fp8_bwd_workspace
-    return f(T, D, F, *codes)
+def _linear_workspace(T: int, D: int, F: int, out_code: int) -> int:
+    _plan(T, F, _blocks(D), out_code, _far(_blocks(D) * BLOCK))
+    return _native.lib().dllm_linear_fp8_workspace(T, D, F, out_code)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bwd_workspace(T: int, D: int, F: int, need_dx: bool, dx_code: int, dw_code: int, ld_wt: int, ld_xt: int) -> int:
+    if need_dx:
+        _plan(T, D, _blocks(F), dx_code, _far(_blocks(F) * BLOCK, ld_wt))
+    _plan(F, D, _blocks(T), dw_code, _far(_blocks(T) * BLOCK, ld_xt))
+    return _native.lib().dllm_linear_fp8_bwd_workspace(T, D, F, dx_code, dw_code, ld_wt, ld_xt)
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -432,7 +453,7 @@ def linear_fp8_bwd(dy: torch.Tensor, saved: LinearFP8, dw: torch.Tensor | None =
         else:
             dw = t
     dy = _rows(dy)
-    n = _linear_workspace(T, D, F, *codes)
+    n = _linear_bwd_workspace(T, D, F, need_dx, *codes, _far(warg[1]), _far(xarg[1]))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = _native.lib().dllm_linear_fp8_bwd(dy.data_ptr(), _native.DT[dy.dtype], dy.stride(0), T, D, F, *xarg, *warg, *args,
