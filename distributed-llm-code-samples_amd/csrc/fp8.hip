@@ -1054,11 +1054,13 @@ static int lin_gemm(const uint8_t* A, long lda, const uint8_t* SA, long ldsa, in
                        ACT_NONE, t & 0xffff, t >> 16, part, stream);
 }
 
-// bytes of workspace of dllm_linear_fp8 (y of type odt) and of dllm_linear_fp8_bwd (dx, dw of types dxdt, dwdt; wt and xt in rows
-// of ldwt and ldxt bytes)
+// bytes of workspace of dllm_linear_fp8 (y of type odt) and of dllm_linear_fp8_bwd (dx, dw of types dxdt, dwdt, dxdt = -1: no dx;
+// wt and xt in rows of ldwt and ldxt bytes)
 long dllm_linear_fp8_workspace(int T, int D, int F, int odt) { return lin_ws(nullptr, T, D, F, D, lin_part(T, F, D, odt, pad_k(D))).bytes; }
 static LinWs lin_bwd_ws(char* base, int T, int D, int F, int dxdt, int dwdt, long ldwt, long ldxt) {
-  return lin_ws(base, T, F, F, T, max(lin_part(T, D, F, dxdt, max(pad_k(F), ldwt)), lin_part(F, D, T, dwdt, max(pad_k(T), ldxt))));
+  const long dw = lin_part(F, D, T, dwdt, max(pad_k(T), ldxt));
+  if (dxdt < 0) return lin_ws(base, 0, 0, F, T, dw);
+  return lin_ws(base, T, F, F, T, max(lin_part(T, D, F, dxdt, max(pad_k(F), ldwt)), dw));
 }
 long dllm_linear_fp8_bwd_workspace(int T, int D, int F, int dxdt, int dwdt, long ldwt, long ldxt) {
   return lin_bwd_ws(nullptr, T, D, F, dxdt, dwdt, ldwt, ldxt).bytes;
@@ -1081,8 +1083,8 @@ int dllm_linear_fp8(const void* x, int xdt, long ldx, const void* w, int wdt, lo
 int dllm_linear_fp8_bwd(const void* dy, int ydt, long ldy, int T, int D, int F, const void* xt, long ldxt, const void* sxt,
                         long ldsxt, int fx, const void* wt, long ldwt, const void* swt, long ldswt, int fw, void* dx, int dxdt,
                         long lddx, void* dw, int dwdt, long lddw, float beta, void* ws, long ws_bytes, void* stream) {
-  if (T <= 0 || D <= 0 || F <= 0 || (dwdt != DT_BF16 && dwdt != DT_F32) || (dxdt != DT_BF16 && dxdt != DT_F32)) return -1;
-  const LinWs l = lin_bwd_ws((char*)ws, T, D, F, dxdt, dwdt, ldwt, ldxt);
+  if (T <= 0 || D <= 0 || F <= 0 || (dwdt != DT_BF16 && dwdt != DT_F32) || (dx && dxdt != DT_BF16 && dxdt != DT_F32)) return -1;
+  const LinWs l = lin_bwd_ws((char*)ws, T, D, F, dx ? dxdt : -1, dwdt, ldwt, ldxt);
   if (ws == nullptr || (uintptr_t)ws % 256 || ws_bytes < l.bytes || dw == nullptr) return -1;
   const long pt = pad_k(T), pf = pad_k(F);
   int rc = dllm_fp8_quantize(dy, ydt, ldy, T, F, dx ? l.a : nullptr, pf, dx ? l.sa : nullptr, T, l.b, pt, l.sb, F, F8_E5M2, F8_E5M2, 0,

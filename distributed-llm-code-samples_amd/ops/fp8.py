@@ -359,8 +359,8 @@ def _linear_workspace(T: int, D: int, F: int, out_code: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_bwd_workspace(T: int, D: int, F: int, need_dx: bool, dx_code: int, dw_code: int, ld_wt: int, ld_xt: int) -> int:
-    if need_dx:
+def _linear_bwd_workspace(T: int, D: int, F: int, dx_code: int, dw_code: int, ld_wt: int, ld_xt: int) -> int:
+    if dx_code >= 0:
         _plan(T, D, _blocks(F), dx_code, _far(_blocks(F) * BLOCK, ld_wt))
     _plan(F, D, _blocks(T), dw_code, _far(_blocks(T) * BLOCK, ld_xt))
     return _native.lib().dllm_linear_fp8_bwd_workspace(T, D, F, dx_code, dw_code, ld_wt, ld_xt)
@@ -436,8 +436,8 @@ def linear_fp8_bwd(dy: torch.Tensor, saved: LinearFP8, dw: torch.Tensor | None =
     codes, args = [], []
     for t, name, shape, dtype in ((dx, "dx", (T, D), dy.dtype), (dw, "dw", (F, D), torch.float32)):
         if name == "dx" and not need_dx:
-            codes.append(0)
-            args += [None, 0, 0]
+            codes.append(-1)
+            args += [None, -1, 0]
             continue
         if t is None:
             t, ld = torch.empty(shape, dtype=dtype, device=dev), D
@@ -453,7 +453,7 @@ def linear_fp8_bwd(dy: torch.Tensor, saved: LinearFP8, dw: torch.Tensor | None =
         else:
             dw = t
     dy = _rows(dy)
-    n = _linear_bwd_workspace(T, D, F, need_dx, *codes, _far(warg[1]), _far(xarg[1]))
+    n = _linear_bwd_workspace(T, D, F, *codes, _far(warg[1]), _far(xarg[1]))
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = _native.lib().dllm_linear_fp8_bwd(dy.data_ptr(), _native.DT[dy.dtype], dy.stride(0), T, D, F, *xarg, *warg, *args,

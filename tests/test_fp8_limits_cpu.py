@@ -23,11 +23,23 @@ def test_far_rows_with_many_on_both_sides_are_refused():
     with pytest.raises(ValueError, match="bytes apart"):
         fp8._linear_workspace(100, FAR, 100, BF16)
     with pytest.raises(ValueError, match="bytes apart"):
-        fp8._linear_bwd_workspace(100, 200, 300, True, BF16, FP32, FAR, 0)
+        fp8._linear_bwd_workspace(100, 200, 300, BF16, FP32, FAR, 0)
     with pytest.raises(ValueError, match="bytes apart"):
-        fp8._linear_bwd_workspace(100, 200, 300, False, BF16, FP32, 0, FAR)
+        fp8._linear_bwd_workspace(100, 200, 300, -1, FP32, 0, FAR)
     assert fp8._linear_workspace(20, FAR, 100, BF16) > 20 * FAR
-    assert fp8._linear_bwd_workspace(100, 200, 300, False, BF16, FP32, FAR, 0) > 0      # (its wᵀ is not read)
+    assert fp8._linear_bwd_workspace(100, 200, 300, -1, FP32, FAR, 0) > 0      # (its wᵀ is not read)
+
+
+def test_backward_without_dx_reserves_nothing_for_it():
+    """The row-wise form of dy (T x F codes and their scales) and dx's K slices are needed for dx only."""
+    def pad(n, to):
+        return -(-n // to) * to
+
+    for T, D, F in ((8192, 4096, 16384), (1000, 512, 1400), (1, 5, 7), (64, 4096, 16384)):
+        columns = pad(F * pad(T, 128), 256) + pad(pad(T, 128) // 128 * F, 256)
+        slices = fp8._plan(F, D, pad(T, 128) // 128, FP32)[1]
+        assert fp8._linear_bwd_workspace(T, D, F, -1, FP32, 0, 0) == columns + (pad(4 * slices * F * D, 256) if slices > 1 else 0)
+        assert fp8._linear_bwd_workspace(T, D, F, BF16, FP32, 0, 0) >= columns + T * pad(F, 128)
 
 
 def test_more_rows_than_a_launch_counts_are_refused():
