@@ -217,3 +217,26 @@ def test_cli_takes_both():
     cfg = config_from_args(make_parser().parse_args(["--optimizer", "muon", "--muon_beta", "0.9", "--fp8", "--dtype", "bf16"]))
     assert cfg.optimizer == "muon" and cfg.muon_beta == 0.9 and cfg.fp8
     assert fp8.BLOCK == 128
+
+
+@pytest.mark.parametrize("act,gated", [("relu", False), ("silu", True)])
+@pytest.mark.parametrize("D,F", [(16, 32), (32, 16)])
+def test_muon_on_transposed_w2_storage(act, gated, D, F):
+    """W2 kept as W2ᵀ: the same update (scale by the logical shape), against the formula and in a checkpoint's logical form."""
+    T, L, lr, wd = 24, 2, 0.02, 0.1
+    layers = _layers(D, F, L, gated)
+    batches = [[b] for b in reference_mock_data([5, 6], T, D)]
+    cfg = TrainConfig(model=ModelConfig(D, F, L, act, gated), batch_size=1, seq_len=T, lr=lr, optimizer="muon", weight_decay=wd,
+                      muon_beta=0.9, w2_storage="transposed")
+    eng = FFNTrainer(cfg, Mesh(), CPU)
+    assert eng.w2t
+    eng.load_full_params(layers)
+    for (x, dy), in batches:
+        eng.train_step(x, dy)
+    want = _muon_oracle(layers, batches, lr, wd, 0.9, True, act)
+    for g, w in zip(eng.gather_full_params(), want):
+        for k in w:
+            # two steps, each off by 3e-4 of its largest singular value (at most 1.25), times the scale sqrt(2) and the learning rate
+            assert g[k].shape == w[k].shape and (g[k].double() - w[k]).abs().max() <= 4 * 3e-4 * 1.25 * 1.5 * lr, k
+    mom = eng.gather_full_params(eng.muon_m)
+    assert all(m["w2"].shape == (D, F) for m in mom)

@@ -162,3 +162,28 @@ def test_graphed_step_refuses():
         eng = FFNTrainer(cfg, Mesh(), torch.device(DEV))
         with pytest.raises(ValueError):
             GraphedStep(eng, 64, 128)
+
+
+@pytest.mark.parametrize("D,F", [(2048, 8192), (8192, 2048)])
+@pytest.mark.parametrize("master", ["split", "fp32"])
+def test_muon_on_transposed_w2_storage(D, F, master):
+    """What a bf16 run of large weights does by itself: W2 stored as W2ᵀ.  One step against the iteration in 64 bits on the
+    engine's own gradient (its momentum after one step from zero)."""
+    from test_muon_step_gpu import iteration, norm, step_tolerance
+
+    T, lr = 512, 0.05
+    layers, (x, dy) = _layers(D, F, 1), _data(T, D)
+    cfg = TrainConfig(model=ModelConfig(D, F, 1), batch_size=1, seq_len=T, lr=lr, dtype="bf16", optimizer="muon",
+                      grad_dtype="fp32", master=master, weight_decay=0.1, w2_storage="transposed")
+    eng = FFNTrainer(cfg, Mesh(), torch.device(DEV))
+    assert eng.w2t
+    eng.load_full_params(layers)
+    eng.train_step(x, dy)
+    grads, got = eng.gather_full_params(eng.muon_m)[0], eng.gather_full_params()[0]
+    for k, w0 in layers[0].items():
+        u = grads[k].to(DEV).double() * (1 + 0.95)           # nesterov: g + beta * momentum, momentum = g
+        o = iteration(u)
+        rate = lr * muon.muon_scale(*w0.shape)
+        want = w0.to(DEV).double() * (1 - lr * 0.1) - rate * o
+        assert got[k].shape == w0.shape
+        assert norm(got[k].to(DEV).double() - want) <= step_tolerance(u, o) * rate * norm(o) + 3 * 2.0 ** -24 * norm(want), k
