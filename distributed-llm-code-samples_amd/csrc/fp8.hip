@@ -345,9 +345,11 @@ __device__ __forceinline__ void f8_epi1(const Fp8GemmArgs& p, int m, int n, floa
 // every sum as it is (jumping over its matrix instructions costs that kernel 270 bytes of spills); an fp32 result jumps over
 // them, as codes times 2^-127 would be rounded to zero in bf16, and infinity times zero is NaN.
 //
-// 8192 x 16384 x 4096 bf16: 444 us (2464 TF; 2898 in a library product without scales).  4096 x 16384 x 8192 fp32 with beta: 925
-// us (1190 TF; 1464 in a library bf16 product).  Bound by the matrix units' power, and at the tile boundary by every block
-// storing at once.
+// 8192 x 16384 x 4096 bf16: 445 us (2470 TF; 2898 in a library product without scales): matrix units busy 62 % of the cycles, at a
+// clock that power holds at 1.9 of 2.4 GHz, and at the tile boundary every block stores at once.  The activation epilogues
+// add the second 268 MB and the function: relu 495, with aux_out 526, dact 559; gelu 591, 601, 643.  4096 x 16384 x 8192 fp32 with
+// beta: 914 us (1200 TF; 1464 in a library bf16 product): matrix units busy half of the cycles at 2.2 GHz, the conversions
+// issue between their instructions.  No LDS conflicts in either.
 // ----------------------------------------------------------------------------------------------
 typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint16_t u16_any __attribute__((aligned(1)));
@@ -760,9 +762,10 @@ __global__ __launch_bounds__(256) void fp8_join(Fp8GemmArgs p) {
 //
 // Fragments go from memory to registers (a step's line of a row is read by the 4 lanes of its row), the waves' sums are
 // added in LDS in the order of the waves.  At one row bound by reading the long operand (16384 x 4096 in 14.7 us, 4.6 TB/s);
-// with more rows by reading the short operand again for every 16 rows of the long one, from L2: 16 rows 19.7 us, 64 rows 46.
+// with more rows by reading the short operand again for every 16 rows of the long one, from L2: 16 rows 19.8 us, 64 rows 46.
 // 64x64 tiles read it once per 64 (19.0 us), so fp8_plan takes them there; on a small long operand they leave CUs empty
-// (1024 x 1024, 64 rows: 5.4 us here, 6.4 there).
+// (1024 x 1024, 64 rows: 5.4 us here, 6.3 there).  A long operand of few rows has too few blocks: one row by 4096 x 16384 takes
+// 19.1 us (256 blocks, 16 steps a wave), by 4096 x 4096 6.2 (floors 13.2 and 3.3).
 // ----------------------------------------------------------------------------------------------
 template <int EPI, typename OutT, int FA, int FB, int MT, bool SWAP>
 __global__ __launch_bounds__(512) void fp8_gemm_rows(Fp8GemmArgs p) {
@@ -902,8 +905,9 @@ constexpr long FP8_PITCH = (0x7fffffffL - 4096) / 256;
 
 // Tile (0: fp8_gemm_rows) and number of K slices: the least time for whole rounds of CUs, in microseconds measured on full
 // rounds: a K step of 128 on one CU (bf16 results / fp32 results), a round's beginning and end, and the slices' partial sums
-// at 1.5 TB/s.  Every choice was measured at six weights (1024 x 1024 to 16384 x 4096) and nine numbers of rows (1 to 256):
-// the one it makes is the fastest or within 13 % of it, and once 23 % (2048 x 8192, 256 rows: 24.8 us, two slices 20.2).
+// at 1.5 TB/s.  Every choice was measured at six weights (1024 x 1024 to 16384 x 4096, both directions), nine numbers of rows (1 to
+// 256) and both result types: the one it makes is the fastest or within 12 % of it in 104 of 108 cases, else 17 to 37 % off
+// (at worst 2048 x 8192, 256 rows, bf16: 24.7 us, four slices of 64 tiles 18.0).
 static void fp8_plan(int M, int N, int nk, bool exact, int& tile, int& ksplit) {
   struct { int ts, blocks; float fast, exact; } kinds[] = {{256, 1, 1.45f, 3.0f}, {128, 1, 0.42f, 0.75f}, {64, 2, 0.30f, 0.40f}};
   float best = 1e30f;

@@ -7,10 +7,11 @@
 //     Q = P_k ... P_1,   A <- (P A) P
 // and X is multiplied by Q once at the end of such a segment.  Segments cost less (for n = 4 m, counting symmetric products
 // half: 19 products of m x m x m for 3 + 2 steps, 32.5 for single steps) and lose digits: a Gram matrix's small eigenvalues
-// are squares of small singular values, and its rounding is amplified as they are (12 a step).  Against 64 bits, errors of
-// gradient-like matrices: single steps 0.5 to 1.1e-6, as an fp32 iteration; 3 + 2 steps 1 to 4e-6; five steps on one Gram
-// matrix 2e-5.  So a result handed out in fp32 runs single steps; a bf16 result (half a step 2e-3) and a weight update
-// (which scales the result by the learning rate before adding it) run segments of three.
+// are squares of small singular values, and its rounding is amplified as they are (12 a step).  Errors against 64 bits, 16 x 16 to
+// 4096 x 16384 (the same iteration in plain fp32): normal matrices 5e-7 to 3e-6 in single steps, 2e-6 to 3e-6 in segments (7e-7 to
+// 9e-6); a few strong directions over noise, singular values over three decades, 4e-6 to 1.6e-5 and 8e-6 to 2.4e-5 (3e-6 to 4e-5).
+// So a result handed out in fp32 runs single steps; a bf16 result (half a step 4e-3) and a weight update (which scales the
+// result by the learning rate before adding it) run segments of three.
 //
 // Every matrix is held as two fp16 planes, v = 2^-s (hi + lo): 22 bits, fp32's to within two.  A product of two such
 // matrices is hi hi + hi lo + lo hi on the fp16 matrix instructions with fp32 accumulation (the missing lo lo is 2^-22 of
@@ -726,7 +727,8 @@ static hipError_t ns_launch(NsGemm p, int B, hipStream_t s) {
   }
   p.ksplit = 1;
   // the tile that needs the least time for whole rounds of CUs: microseconds of a 64-deep K step on one CU (measured on full
-  // rounds: 128 x 128 is bound by LDS, the larger ones by the matrix units' power), and of a round's beginning and end
+  // rounds: 128 x 128 is bound by LDS, 256 x 256 by the matrix units' power, busy 80 to 85 % of the cycles at 1.7 GHz, 192 x 192
+  // half by it, 50 to 54 % at 2.0), and of a round's beginning and end
   const long cus = cu_count();
   const float steps = 3.f * (float)(p.K >> 6);
   auto time = [&](int ts, long per_cu, float step) {
