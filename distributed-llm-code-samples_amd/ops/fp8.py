@@ -194,6 +194,8 @@ def quantize_fp8_both(x: torch.Tensor, fmt: str = "e4m3", fmt_t: str = "e4m3", *
     R, C = _shape2(x)
     out, arg = _target(out, R, C, fmt, x.device, "out")
     out_t, arg_t = _target(out_t, C, R, fmt_t, x.device, "out_t")
+    if R and C and (arg[0] == arg_t[0] or arg[2] == arg_t[2]):   # both orientations are written at once
+        raise ValueError("out and out_t must not share memory")
     _quantize(x, R, C, out, arg, out_t, arg_t, tile)
     return out, out_t
 

@@ -1,5 +1,6 @@
 """Sizes and row strides at the end of what the 8-bit products take: another kernel, or a refusal by name."""
 import pytest
+import torch
 
 from dllm.ops import fp8
 
@@ -54,3 +55,14 @@ def test_pitch_limit_is_the_fetches_reach():
     """256 rows, and what one step of 128 bytes adds, stay below 2^31 bytes from the first."""
     assert 256 * fp8.MAX_PITCH + 4096 <= 2 ** 31 - 1 < 256 * (fp8.MAX_PITCH + 1) + 4096
     assert fp8._far(fp8.MAX_PITCH, 5) == 0 and fp8._far(7, FAR) == FAR
+
+
+def test_one_target_for_both_orientations_is_refused():
+    x, out, other = torch.randn(40, 40), fp8.fp8_empty(40, 40), fp8.fp8_empty(40, 40)
+    for out_t in (out, out._replace(data=other.data), out._replace(scale=other.scale)):
+        with pytest.raises(ValueError, match="share memory"):
+            fp8.quantize_fp8_both(x, out=out, out_t=out_t)
+    q, qt = fp8.quantize_fp8_both(x, out=out, out_t=other)
+    assert torch.equal(fp8.dequantize_fp8(qt), fp8.dequantize_fp8(fp8.quantize_fp8(x.t())))
+    none, none_t = fp8.quantize_fp8_both(torch.empty(0, 0))
+    assert none.rows == none_t.rows == 0

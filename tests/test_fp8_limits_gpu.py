@@ -60,3 +60,19 @@ def test_linear_of_very_long_rows():
     assert ((y.double() - want).abs() <= (7 * 2.0 ** -13 + D / 256 * 2.0 ** -24) * mag + 2.0 ** -8 * want.abs()).all()
     with pytest.raises(ValueError, match="bytes apart"):
         fp8.linear_fp8(w, w)
+
+
+@pytest.mark.parametrize("tile", [(256, 1), (128, 1), (64, 2)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_farthest_rows_of_the_tiles(monkeypatch, tile, out):
+    """Row strides at the limit: a tile's last row lies just below 2^31 bytes from its first."""
+    pitch = fp8.MAX_PITCH // 128 * 128
+    a, b = fp8.quantize_fp8(rand(300, 512, 1).to(DEV), "e5m2"), fp8.quantize_fp8(rand(270, 512, 2).to(DEV))
+    monkeypatch.setattr(fp8, "_plan", lambda *_: tile)
+    want = fp8.gemm_fp8(a, b, out_dtype=out)
+    wide = []
+    for q in (a, b):
+        buf = torch.empty(q.rows, pitch, dtype=q.data.dtype, device=DEV)
+        buf[:, :512].copy_(q.data)
+        wide.append(fp8.BlockFP8(buf[:, :512], q.scale, q.k))
+    assert torch.equal(fp8.gemm_fp8(wide[0], wide[1], out_dtype=out), want)
